@@ -38,7 +38,9 @@ typedef enum {
 
 typedef void *jas_stream_t;
 
-typedef enum { JAS_F32 = 0, JAS_F64 = 1, JAS_I32 = 2, JAS_BF16 = 3 } jas_dtype;
+/* JAS_I8 and JAS_F8E4M3 (OCP e4m3: no infinities, largest value 448) are storage types of the
+ * paged cache only. */
+typedef enum { JAS_F32 = 0, JAS_F64 = 1, JAS_I32 = 2, JAS_BF16 = 3, JAS_I8 = 4, JAS_F8E4M3 = 5 } jas_dtype;
 
 /* ------------------------------------------------------------------ runtime */
 /* Device selection and library stream creation.  Storage behind mat_t<T>
@@ -264,6 +266,65 @@ jas_status jas_attn_decode_noalloc(const float *d_q, const float *d_K, const flo
                                    const int32_t *d_seqlens, int B, int H, int D, int max_len,
                                    long k_sb, long k_sh, float scale, jas_stream_t stream);
 
+/* ------------------------------------------------------------------ paged key/value cache */
+/* No counterpart in the reference (jasmine recomputes the whole prefix each step,
+ * transformer_test.hpp:231-238): the cache and the attention of a server whose sequences grow
+ * and end on their own.  Two pools of n_pages pages of page_size tokens each; element d of head
+ * h of slot s of page p is pool[p * page_stride + h * head_stride + s * tok_stride + d], strides
+ * in elements, the same for keys and values, each a multiple of 16 bytes, as the pools' addresses
+ * are.  Position t of sequence b lies in slot t % page_size of page
+ * d_table[b * table_stride + t / page_size].  An entry outside [0, n_pages) is no page: nothing
+ * is written to it, reading it back gives zeros, and attention takes its keys as masked.
+ *
+ * dtype JAS_F32, JAS_BF16, JAS_I8 or JAS_F8E4M3.  The 8-bit types hold a row of dh values as
+ * codes and one fp32 scale at d_k_scale / d_v_scale[(p * n_kv + h) * page_size + s]:
+ * scale = max |x| / 127 (JAS_I8) or / 448 (JAS_F8E4M3), rounded to fp32; code = x / scale,
+ * rounded once, to nearest even; the row's value is code * scale.  A row whose scale would be
+ * below 2^-126 has scale 0 and reads as zeros; a row with an infinity or NaN has scale NaN and
+ * reads as NaN.  dh in {32, 64, 128}. */
+typedef struct {
+    void *d_k, *d_v;
+    float *d_k_scale, *d_v_scale;  /* 8-bit types only */
+    const int32_t *d_table;
+    int64_t page_stride, head_stride, tok_stride;
+    int32_t table_stride, max_pages; /* entries from one sequence's row to the next; entries of a row */
+    int32_t dtype, n_pages, page_size, n_kv, dh;
+} jas_paged_kv;
+
+/* A ragged batch: of n rows of tokens, rows d_cu[b] .. d_cu[b + 1] - 1 are the last tokens of
+ * sequence b, which has d_lens[b] tokens with them (d_cu: B + 1 non-decreasing device int32 from
+ * 0; d_lens: B).  Row i of sequence b so stands at position d_lens[b] - d_cu[b + 1] + i.  Rows
+ * from d_cu[B] on are not read and not written.  Positions below 0 or past the table's row are
+ * no tokens: not written, read as zeros.
+ *
+ * Writes the new tokens' keys and values (device, JAS_F32 or JAS_BF16, token stride st, head
+ * stride sh, in elements, both tensors alike) to the cache.  Two rows of one call must not name
+ * the same slot (a page that two sequences share is written by one of them at most). */
+jas_status jas_kv_append(const jas_paged_kv *kv, const void *d_k, const void *d_v, int n, int64_t st, int64_t sh,
+                         int B, const int32_t *d_cu, const int32_t *d_lens, int dtype, jas_stream_t stream);
+/* Reads them back, widened or rounded to dtype (JAS_F32 or JAS_BF16).  d_cu may count whole
+ * sequences.  Either output may be NULL. */
+jas_status jas_kv_read(const jas_paged_kv *kv, void *d_k, void *d_v, int n, int64_t st, int64_t sh, int B,
+                       const int32_t *d_cu, const int32_t *d_lens, int dtype, jas_stream_t stream);
+
+/* Attention of the batch's rows over the cache, which holds their own keys and values already:
+ * O = softmax(scale Q K^T) V over the keys at positions up to the row's own (causal = 1) or over
+ * all of its sequence (0).  One row per sequence is a decode step, more a chunk of a prompt; both
+ * may be mixed in a call.  Query head h of H reads key head h / (H / n_kv).  Q and O: row stride
+ * st, head stride sh (elements); O must not overlap Q.  A row that sees no key is zeros.  Keys
+ * past a row's position do not reach it, whatever they hold.
+ * dtype JAS_F32 (over a cache of any type: fp32 accuracy) or JAS_BF16 (over JAS_BF16, JAS_I8 and
+ * JAS_F8E4M3; probabilities rounded to bf16, sums in fp32).
+ * max_q: new tokens of the longest sequence, max_len: tokens of the longest (hosts' numbers, so
+ * that the call reads nothing back; max_q only picks the kernel, lengths above max_len are taken
+ * as max_len).  d_work: jas_attn_paged_workspace(...) bytes of the same arguments, 16-byte
+ * aligned, no initialisation, NULL where that is 0; calls that share it must not overlap. */
+size_t jas_attn_paged_workspace(int n, int B, int H, int n_kv, int dh, int max_q, int max_len);
+jas_status jas_attn_paged(const void *d_q, void *d_o, const jas_paged_kv *kv, int n, int B, const int32_t *d_cu,
+                          const int32_t *d_lens, int H, int max_q, int max_len, int64_t q_st, int64_t q_sh,
+                          int64_t o_st, int64_t o_sh, float scale, int causal, int dtype, void *d_work,
+                          jas_stream_t stream);
+
 /* ------------------------------------------------------------------ RoPE, embeddings, argmax */
 /* jasmine RoPE_net_t::forward (mat_RoPE_t.hpp:166-188) with mat_RoPE_t::init angles
  * (mat_RoPE_t.hpp:107-131); x, y row-major [d, T] feature-major. */
@@ -273,11 +334,54 @@ jas_status jas_rope_jasmine_f64(const double *d_x, double *d_y, int d, int T, ja
  * positions pos[n] (device int32), nh heads of dh each, token stride tstride elements. */
 jas_status jas_rope_llama(float *d_x, const int32_t *d_pos, int n, int nh, int dh, long tstride,
                           float theta, jas_stream_t stream);
+/* Rotary positions in general (new): the first rot of each head's dh elements turn, the others
+ * are copied.  Pair i turns by pos[n] * freq[i] radians, cos and sin times mscale.  layout
+ * JAS_ROPE_PAIRS: elements (2i, 2i + 1), as jas_rope_llama; JAS_ROPE_HALVES: (i, i + rot / 2).
+ * x, y: token stride st, head stride sh (elements; a fused QKV row is one token of all its query
+ * and key heads); dtype JAS_F32 or JAS_BF16.  y may be x itself with the same strides; any other
+ * overlap is not allowed.  d_freq: rot / 2 doubles on the device, as jas_rope_freqs makes them
+ * or the caller's own; angles are formed and reduced in 64 bits, so far positions keep theirs. */
+typedef enum { JAS_ROPE_PAIRS = 0, JAS_ROPE_HALVES = 1 } jas_rope_layout;
+jas_status jas_rope(const void *d_x, void *d_y, const int32_t *d_pos, const double *d_freq, int n, int nh, int dh,
+                    int rot, int64_t x_st, int64_t x_sh, int64_t y_st, int64_t y_sh, int layout, float mscale,
+                    int dtype, jas_stream_t stream);
+/* Frequencies for a context longer than the orig_ctx positions that a model was trained on (host
+ * only, no device call).  f_i = theta^(-2i / rot), then
+ * JAS_ROPE_SCALE_LINEAR: f / factor;
+ * JAS_ROPE_SCALE_YARN: f / factor for pairs that turn less than `low` times over orig_ctx, f for
+ *   those that turn more than `high` times, a ramp over the pair index between the two (its ends
+ *   rounded outwards to whole indexes); *h_mscale = 0.1 ln(factor) + 1 for factor > 1;
+ * JAS_ROPE_SCALE_BANDS: f / factor where orig_ctx f / (2 pi) is below low, f above high, between
+ *   them interpolated linearly in that number of turns.
+ * h_freq: rot / 2 doubles; h_mscale (1 but for YARN) may be NULL; scaling NULL: none. */
+typedef enum { JAS_ROPE_SCALE_NONE = 0, JAS_ROPE_SCALE_LINEAR = 1, JAS_ROPE_SCALE_YARN = 2, JAS_ROPE_SCALE_BANDS = 3 } jas_rope_scale;
+typedef struct {
+    int32_t kind, orig_ctx;
+    double factor, low, high;
+} jas_rope_scaling;
+jas_status jas_rope_freqs(int rot, double theta, const jas_rope_scaling *scaling, double *h_freq, float *h_mscale);
 /* out[n][d] = wte[ids[n]] (+ wpe[pos[n]] if d_wpe) -- token embedding gather (new) */
 jas_status jas_embed(const float *d_wte, const float *d_wpe, const int32_t *d_ids, const int32_t *d_pos,
                      float *d_out, int n, int d, jas_stream_t stream);
 /* argmax over each of n rows of length V (first maximum wins) */
 jas_status jas_argmax(const float *d_x, int n, int V, long ld, int32_t *d_out, jas_stream_t stream);
+/* One token for each of n rows of V logits (JAS_F32 or JAS_BF16, leading dimension ld), beside
+ * jas_argmax (new).  w_i = exp((x_i - max x) / temperature).  Kept are, of the row in order of
+ * falling value, lowest index first among equals: the first top_k (0 or less: all); of those the
+ * shortest run from the first whose w reach top_p of their sum (1 or more: all; the first is
+ * always kept); and of those the ones with w >= min_p (above 1: as 1).  The token is the lowest
+ * index whose running sum of kept w, in index order, exceeds u times their sum; u[n] in [0, 1)
+ * is the caller's (outside it, or NaN: the nearer end, 0).  temperature 0 or less or NaN: the
+ * first maximum.  NaN logits count as -inf; +inf ones share the whole weight.  A row with nothing above
+ * -inf gives id -1 and logp -inf.  logp (may be NULL): log of the token's share of the kept w.
+ * d_temp, d_top_k, d_top_p, d_min_p: one value a row, each may be NULL (1, 0, 1, 0).
+ * Weights are formed in 64 bits and summed as whole numbers, so results do not depend on the
+ * order of sums.  V up to 2^22.  d_work: jas_sample_workspace(n, V) bytes, 16-byte aligned, no
+ * initialisation, NULL where that is 0; calls that share it must not overlap. */
+size_t jas_sample_workspace(int n, int V);
+jas_status jas_sample(const void *d_x, int n, int V, int64_t ld, const float *d_temp, const int32_t *d_top_k,
+                      const float *d_top_p, const float *d_min_p, const float *d_u, int32_t *d_ids, float *d_logp,
+                      int dtype, void *d_work, jas_stream_t stream);
 /* Seeded N(mean, std) fill, same counter-based generator as the host side. */
 jas_status jas_fill_normal(float *d_x, size_t n, uint64_t seed, uint64_t stream_id, float mean, float std,
                            jas_stream_t stream);

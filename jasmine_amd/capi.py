@@ -19,7 +19,9 @@ IP = C.POINTER(C.c_int32)
 L = C.c_long
 I = C.c_int
 
-JAS_F32, JAS_F64, JAS_I32, JAS_BF16 = 0, 1, 2, 3
+JAS_F32, JAS_F64, JAS_I32, JAS_BF16, JAS_I8, JAS_F8E4M3 = 0, 1, 2, 3, 4, 5
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN, ROPE_SCALE_BANDS = 0, 1, 2, 3
 ERR_NAMES = {1: "invalid argument", 2: "runtime error", 3: "HIP error", 4: "out of memory", 5: "out of range"}
 
 
@@ -46,6 +48,19 @@ class LmConfig(C.Structure):
                 ("eps", C.c_float), ("rope_theta", C.c_float), ("weight_bf16", C.c_int32), ("kv_bf16", C.c_int32)]
 
 
+class PagedKv(C.Structure):
+    """jas_paged_kv: the pools, scales, table and layout of a paged key/value cache."""
+    _fields_ = [("d_k", VP), ("d_v", VP), ("d_k_scale", VP), ("d_v_scale", VP), ("d_table", VP),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("tok_stride", C.c_int64),
+                ("table_stride", C.c_int32), ("max_pages", C.c_int32), ("dtype", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv", C.c_int32), ("dh", C.c_int32)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("orig_ctx", C.c_int32), ("factor", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+L64 = C.c_int64
 _sigs = {
     "jas_init": [I], "jas_malloc": [C.POINTER(VP), C.c_size_t], "jas_free": [VP],
     "jas_memset": [VP, I, C.c_size_t, VP], "jas_memcpy_h2d": [VP, VP, C.c_size_t, VP],
@@ -67,6 +82,12 @@ _sigs = {
     "jas_attn_prefill": [VP, VP, VP, VP, I, I, I, I, I, L, L, L, L, L, L, L, L, L, C.c_float, I, I, VP],
     "jas_attn_decode": [VP, VP, VP, VP, VP, I, I, I, I, L, L, C.c_float, VP, VP],
     "jas_attn_decode_noalloc": [VP, VP, VP, VP, VP, I, I, I, I, L, L, C.c_float, VP],
+    "jas_kv_append": [C.POINTER(PagedKv), VP, VP, I, L64, L64, I, VP, VP, I, VP],
+    "jas_kv_read": [C.POINTER(PagedKv), VP, VP, I, L64, L64, I, VP, VP, I, VP],
+    "jas_attn_paged": [VP, VP, C.POINTER(PagedKv), I, I, VP, VP, I, I, I, L64, L64, L64, L64, C.c_float, I, I, VP, VP],
+    "jas_rope": [VP, VP, VP, VP, I, I, I, I, L64, L64, L64, L64, I, C.c_float, I, VP],
+    "jas_rope_freqs": [I, C.c_double, C.POINTER(RopeScaling), C.POINTER(C.c_double), FP],
+    "jas_sample": [VP, I, I, L64, VP, VP, VP, VP, VP, VP, VP, I, VP, VP],
     "jas_rope_jasmine": [VP, VP, I, I, VP],
     "jas_rope_jasmine_f64": [VP, VP, I, I, VP],
     "jas_rope_llama": [VP, VP, I, I, I, L, C.c_float, VP],
@@ -103,6 +124,10 @@ lib.jas_attn_decode_workspace.restype = C.c_size_t
 lib.jas_attn_decode_workspace.argtypes = [I, I, I, I]
 lib.jas_attn_decode_scratch_max.restype = C.c_size_t
 lib.jas_attn_decode_scratch_max.argtypes = []
+lib.jas_attn_paged_workspace.restype = C.c_size_t
+lib.jas_attn_paged_workspace.argtypes = [I, I, I, I, I, I, I]
+lib.jas_sample_workspace.restype = C.c_size_t
+lib.jas_sample_workspace.argtypes = [I, I]
 lib.jas_lm_position.restype = I
 lib.jas_lm_position.argtypes = [VP]
 lib.jas_lm_attn_splits.restype = I
@@ -113,7 +138,7 @@ lib.jas_lm_stream.argtypes = [VP]
 # every symbol the C header declares (checked by the CPU test that the library exports them)
 EXPORTED = sorted(list(_sigs) + ["jas_last_error", "jas_version", "jas_default_stream",
                                  "jas_attn_decode_workspace", "jas_attn_decode_scratch_max", "jas_ew_jit_mode", "jas_lm_position", "jas_lm_stream",
-                                 "jas_lm_attn_splits"])
+                                 "jas_lm_attn_splits", "jas_attn_paged_workspace", "jas_sample_workspace"])
 
 
 def check(code):
@@ -175,6 +200,14 @@ def leaf(arr, rows=None, cols=None, row_first=1, roff=0, coff=0, transposed=0, v
     vr = vrows if vrows is not None else (c - coff if transposed else r - roff)
     vc = vcols if vcols is not None else (r - roff if transposed else c - coff)
     return Leaf(arr.ptr, _DT[arr.dtype], r, c, row_first, roff, coff, transposed, vr, vc)
+
+
+def rope_freqs(rot, theta, scaling=None):
+    """(frequencies as float64 [rot / 2], magnitude of cos and sin) for jas_rope."""
+    f, m = np.empty(max(rot, 0) // 2, np.float64), C.c_float()
+    check(lib.jas_rope_freqs(rot, theta, C.byref(scaling) if scaling is not None else None,
+                             f.ctypes.data_as(C.POINTER(C.c_double)), C.byref(m)))
+    return f, m.value
 
 
 class Lm:
