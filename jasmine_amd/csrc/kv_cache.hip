@@ -38,7 +38,7 @@ jas_status paged_view(const jas_paged_kv *kv, PagedView &v, const char *who)
     v.page_stride = kv->page_stride, v.head_stride = kv->head_stride, v.tok_stride = kv->tok_stride;
     v.table_stride = kv->table_stride, v.n_pages = kv->n_pages, v.page_size = kv->page_size, v.n_kv = kv->n_kv;
     const long cap = (long)kv->max_pages * kv->page_size;
-    v.cap = (int)(cap < 0x7fffffffl ? cap : 0x7fffffffl);
+    v.cap = (int)(cap < 0x7fff0000l ? cap : 0x7fff0000l);  // (a tile past the end stays below 2^31)
     v.by_page.set((uint32_t)kv->page_size);
     return JAS_OK;
 }
