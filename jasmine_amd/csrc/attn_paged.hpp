@@ -36,14 +36,15 @@ struct PagedAttnArgs {
     long q_st, q_sh, o_st, o_sh;
     float scale_log2;
     int q_vec, o_vec;           // rows of Q, O start on 16 bytes
-    int tiles, nsplit;          // grid: tiles x nsplit x key heads
+    int tiles, nsplit, chunk;   // grid: tiles x nsplit x key heads; keys of a split, at least
+    int sorted, cus;            // tiles in order of falling length; compute units
     float *part;                // nsplit > 1: rows of D means, then exponent base and sum
 };
 
 // How a call is launched
 struct PagedPlan {
     int rows;  // of a tile: 16 (its waves share the keys), 64 or 128
-    int tiles, nsplit;
+    int tiles, nsplit, chunk;
 };
 // One call's kernels for head dim 32, 64, 128
 void paged_launch_32(const PagedAttnArgs &p, int rows, int cache, int dtype, hipStream_t s);
@@ -70,42 +71,86 @@ __device__ __forceinline__ float paged_sum_rows(float v)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Sequence b of the batch: its rows, and its length with them
+// A sequence of the batch: its rows, and its length with them
 struct PagedSeq {
     int row0, rows, len;
 };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs &p, int b)
-{
-    PagedSeq s;
-    s.row0 = max(0, min(p.bt.cu[b], p.bt.n));
-    s.rows = max(0, min(p.bt.cu[b + 1], p.bt.n) - s.row0);
-    s.len = max(0, min(p.bt.lens[b], min(p.kv.cap, p.max_len)));
-    return s;
-}
 
 // Tile x of the grid: sequence b owns tiles from floor(cu[b] G / M) + b on, at least as many as
-// its rows fill, so a count of the sequences that start at or below x finds it (one load a
-// thread and no running sum).  Returns its tile number in b; the count is over the workgroup.
+// its rows fill, so the thread that holds b knows it from cu[b] and cu[b + 1] alone: one round of
+// loads, no running sum.  Returns x's tile number in b, or -1.  By the whole workgroup.
 template <int M>
-__device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b)
+__device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
 {
-    int count = 0;
+    __shared__ int s_b, s_seq[4];
+    if (threadIdx.x == 0) s_b = -1, s_seq[3] = -1;
+    __syncthreads();
+    int own = -2, row0 = 0, rows = 0, len = 0, at = 0;
     for (int j0 = 0; j0 < p.bt.B; j0 += 256) {
         const int j = j0 + (int)threadIdx.x;
-        const bool at = j < p.bt.B && (long)max(0, min(p.bt.cu[j], p.bt.n)) * p.G / M + j <= x;
-        count += __syncthreads_count(at);
+        if (j >= p.bt.B) break;
+        const int c0 = max(0, min(p.bt.cu[j], p.bt.n)), c1 = max(c0, min(p.bt.cu[j + 1], p.bt.n)), n = p.bt.lens[j];
+        const int first = (int)((long)c0 * p.G / M + j);
+        if (first <= x && (j + 1 == p.bt.B || (int)((long)c1 * p.G / M + j + 1) > x))
+            own = j, row0 = c0, rows = c1 - c0, len = n, at = x - first;
     }
-    b = max(0, count - 1);
-    return x - (int)((long)max(0, min(p.bt.cu[b], p.bt.n)) * p.G / M + b);
+    if (own >= 0) s_b = own;  // (one thread's, where cu does not fall)
+    __syncthreads();
+    if (own == s_b) s_seq[0] = row0, s_seq[1] = rows, s_seq[2] = max(0, min(len, min(p.kv.cap, p.max_len))), s_seq[3] = at;
+    __syncthreads();
+    b = max(0, s_b);
+    sq.row0 = s_seq[0], sq.rows = s_seq[1], sq.len = s_seq[2];
+    return s_seq[3];
 }
 
-// Where key t of sequence b lies: its page (-1: none) and slot
-__device__ __forceinline__ int paged_page(const PagedAttnArgs &p, int b, int t, int &slot)
+// The same in order of falling length, for launches whose workgroups own whole sequences of keys (B
+// <= 256): each thread adds the tiles of the sequences before its own.  Workgroups start in the order
+// of their ids, i and i + C (C compute units) on one unit where two fit, so the second C of them
+// are taken from the light end: 8 chunks of up to 256 beside 16 decoding sequences, 148 -> 122 us.
+template <int M>
+__device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
+{
+    __shared__ int s_tiles[256], s_len[256], s_seq[4];
+    const int j = threadIdx.x;
+    int row0 = 0, rows = 0, len = 0;
+    if (j < p.bt.B) {
+        row0 = max(0, min(p.bt.cu[j], p.bt.n));
+        rows = max(0, min(p.bt.cu[j + 1], p.bt.n) - row0);
+        len = max(0, min(p.bt.lens[j], min(p.kv.cap, p.max_len)));
+    }
+    const int tiles = (int)(((long)rows * p.G + M - 1) / M);
+    s_tiles[j] = tiles, s_len[j] = len;
+    if (j == 0) s_seq[3] = -1;
+    __syncthreads();
+    int first = 0, total = 0;
+    for (int k = 0; k < p.bt.B; ++k) {
+        const int t = s_tiles[k], n = s_len[k];
+        total += t;
+        first += n > len || (n == len && k < j) ? t : 0;
+    }
+    const int lo = p.cus / p.kv.n_kv, hi = min(2 * lo, total);  // tiles of the first and second round
+    if (x >= lo && x < hi) x = lo + hi - 1 - x;
+    if (x >= first && x < first + tiles) s_seq[0] = row0, s_seq[1] = rows, s_seq[2] = len, s_seq[3] = x - first, s_tiles[0] = j;
+    __syncthreads();
+    sq.row0 = s_seq[0], sq.rows = s_seq[1], sq.len = s_seq[2];
+    b = max(0, min(s_tiles[0], p.bt.B - 1));
+    return s_seq[3];
+}
+
+// Keys [k_lo, k_hi) of a split: p.chunk of them, or as many as nsplit splits need to cover kend
+__device__ __forceinline__ void paged_split(const PagedAttnArgs &p, int kend, int split, int &k_lo, int &k_hi)
+{
+    const int per = max(p.chunk, ((kend + p.nsplit - 1) / p.nsplit + 127) / 128 * 128);
+    k_lo = (int)min((long)kend, (long)split * per);
+    k_hi = min(kend, k_lo + per);
+}
+
+// Where key t of sequence b lies: the table's entry for its page, and the slot
+__device__ __forceinline__ int paged_entry(const PagedAttnArgs &p, int b, int t, int &slot)
 {
     const int q = (int)p.kv.by_page.div((uint32_t)t);
     slot = t - q * p.kv.page_size;
-    const int page = p.kv.table[(long)b * p.kv.table_stride + q];
-    return page >= 0 && page < p.kv.n_pages ? page : -1;
+    return p.kv.table[(long)b * p.kv.table_stride + q];
 }
 
 template <int CK>
@@ -122,7 +167,7 @@ __device__ __forceinline__ float cache_value(const void *pool, long at)
 // out: elements lane + 64 e of the weighted mean of the values.  A mean of numbers near the end
 // of fp32 is one itself though their sum is not: acc2 adds them times 2^-32.
 template <int D, int CK, typename T>
-__device__ __attribute__((noinline)) void paged_row(const PagedAttnArgs &p, int b, int hk, const T *q, int k_lo, int k_hi,
+__device__ __forceinline__ void paged_row(const PagedAttnArgs &p, int b, int hk, const T *q, int k_lo, int k_hi,
                                                     float &m, float &l, float (&out)[(D + 63) / 64])
 {
     const int lane = threadIdx.x & 63;
@@ -134,8 +179,8 @@ __device__ __attribute__((noinline)) void paged_row(const PagedAttnArgs &p, int 
     for (int k0 = k_lo; k0 < k_hi; k0 += 64) {
         const int t = k0 + lane;
         int slot = 0, page = -1;
-        if (t < k_hi) page = paged_page(p, b, t, slot);
-        const bool sees = page >= 0;
+        if (t < k_hi) page = paged_entry(p, b, t, slot);
+        const bool sees = page >= 0 && page < p.kv.n_pages;
         const long at = (long)page * p.kv.page_stride + hk * p.kv.head_stride + slot * p.kv.tok_stride;
         const long sc = ((long)page * p.kv.n_kv + hk) * p.kv.page_size + slot;
         float s = -INFINITY, vs = 1.f;
@@ -199,7 +244,7 @@ __device__ __forceinline__ PagedRow paged_row_of(const PagedAttnArgs &p, const P
 
 // Computes the rows of a tile again whose bit in bad[] is set: results or partial results
 template <int D, int CK, typename T>
-__device__ __attribute__((noinline)) void paged_again(const PagedAttnArgs &p, int b, int hk, const PagedSeq &sq, int r0, int rows,
+__device__ __forceinline__ void paged_again(const PagedAttnArgs &p, int b, int hk, const PagedSeq &sq, int r0, int rows,
                                                       const unsigned *bad, int k_lo, int k_hi, float *part)
 {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -222,6 +267,11 @@ __device__ __attribute__((noinline)) void paged_again(const PagedAttnArgs &p, in
 // Raw registers of 32 d of a key row, in the order of K's operand: lane (row r16, group g) slot
 // j holds d = 32 c + 8 g + j (bf16), 32 c + 4 g + j and 32 c + 16 + 4 g + j - 4 (fp32), and with codes
 // the 64 d of two steps lie 16 a lane: 64 (c / 2) + 16 g + 8 (c % 2) + j (D = 32: as bf16).
+template <bool NT, typename V>
+__device__ __forceinline__ V cache_load(const void *p)
+{
+    return NT ? __builtin_nontemporal_load((const V *)p) : *(const V *)p;
+}
 template <int D, int CK>
 struct KOperand {
     static constexpr int CD = D / 32, RW = CK == CK_F32 ? 8 : CK == CK_BF16 ? 4 : 2;
@@ -231,31 +281,32 @@ struct KOperand {
         if (CK == CK_BF16 || D == 32) return 32 * c + 8 * g + j;
         return 64 * (c / 2) + 16 * g + 8 * (c % 2) + j;
     }
-    // row: the first element of the key
+    // row: the first element of the key; NT: a stream that is read once
+    template <bool NT = false>
     static __device__ __forceinline__ void load(const void *row, int g, uint32_t (&r)[CD][RW])
     {
         const char *p = (const char *)row + (CK == CK_F32 || CK == CK_BF16 || D >= 64 ? 16 : 8) * g;
         if constexpr (CK == CK_F32) {
 #pragma unroll
             for (int c = 0; c < CD; ++c) {
-                const u32x4 a = *(const u32x4 *)(p + 128 * c), b = *(const u32x4 *)(p + 128 * c + 64);
+                const u32x4 a = cache_load<NT, u32x4>((p + 128 * c)), b = cache_load<NT, u32x4>((p + 128 * c + 64));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) r[c][e] = a[e], r[c][4 + e] = b[e];
             }
         } else if constexpr (CK == CK_BF16) {
 #pragma unroll
             for (int c = 0; c < CD; ++c) {
-                const u32x4 a = *(const u32x4 *)(p + 64 * c);
+                const u32x4 a = cache_load<NT, u32x4>((p + 64 * c));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) r[c][e] = a[e];
             }
         } else if constexpr (D == 32) {
-            const u32x2 a = *(const u32x2 *)p;
+            const u32x2 a = cache_load<NT, u32x2>(p);
             r[0][0] = a[0], r[0][1] = a[1];
         } else {
 #pragma unroll
             for (int c = 0; c < CD; c += 2) {
-                const u32x4 a = *(const u32x4 *)(p + 32 * c);
+                const u32x4 a = cache_load<NT, u32x4>((p + 32 * c));
                 r[c][0] = a[0], r[c][1] = a[1], r[c + 1][0] = a[2], r[c + 1][1] = a[3];
             }
         }
@@ -297,17 +348,18 @@ __device__ __forceinline__ void k_planes(const uint32_t (&r)[RW], u32x4 (&pl)[NK
 template <int CK, int EV>
 struct VOperand {
     static constexpr int BYTES = EV * cache_bytes<CK>, RW = BYTES < 4 ? 1 : BYTES / 4;
+    template <bool NT = false>
     static __device__ __forceinline__ void load(const void *p, uint32_t (&r)[RW])
     {
-        if constexpr (BYTES == 2) r[0] = *(const uint16_t *)p;
-        else if constexpr (BYTES == 4) r[0] = *(const uint32_t *)p;
+        if constexpr (BYTES == 2) r[0] = cache_load<NT, uint16_t>(p);
+        else if constexpr (BYTES == 4) r[0] = cache_load<NT, uint32_t>(p);
         else if constexpr (BYTES == 8) {
-            const u32x2 a = *(const u32x2 *)p;
+            const u32x2 a = cache_load<NT, u32x2>(p);
             r[0] = a[0], r[1] = a[1];
         } else {
 #pragma unroll
             for (int k = 0; k < RW; k += 4) {
-                const u32x4 a = *(const u32x4 *)((const char *)p + 4 * k);
+                const u32x4 a = cache_load<NT, u32x4>((const char *)p + 4 * k);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) r[k + e] = a[e];
             }
@@ -412,8 +464,13 @@ __device__ __forceinline__ void q_planes(const T *q, bool there, int g, bool vec
 // turn and keep a softmax each, joined at the end.  Nothing goes through LDS on the way: K and V
 // are read from memory in operand order (each 16-lane group reads whole value rows, 64-byte
 // pieces of key rows), V is transposed by v_perm in the lane that read it.
+// Waves a SIMD: loads in flight hide the memory's latency, as many as registers hold (fp32 rows keep
+// three planes of Q, fp32 caches twice the raw words)
 template <int D, int CK, typename T>
-__global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p)
+constexpr int stream_waves = D == 128 ? (sizeof(T) == 2 ? 3 : CK == CK_F32 ? 1 : 2) : CK == CK_F32 ? 2 : 3;
+
+template <int D, int CK, typename T>
+__global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_kernel(const PagedAttnArgs p)
 {
     constexpr int M = 16, CD = D / 32, EV = D / 16, NP = sizeof(T) == 4 ? 3 : 1, NK = CK == CK_F32 ? 3 : 1;
     using KO = KOperand<D, CK>;
@@ -429,15 +486,20 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hk = blockIdx.x % p.kv.n_kv, rest = blockIdx.x / p.kv.n_kv, split = rest % p.nsplit, x = rest / p.nsplit;
     int b;
-    const int tile = paged_tile<M>(p, x, b);
-    const PagedSeq sq = paged_seq(p, b);
+    PagedSeq sq;
+    const int tile = paged_tile<M>(p, x, b, sq);
     const int r0 = tile * M, rows = min(M, sq.rows * p.G - r0);
     if (tile < 0 || rows <= 0) return;
     const PagedRow row = paged_row_of(p, sq, hk, r0 + min(r16, rows - 1));
     const int kend = paged_row_of(p, sq, hk, r0 + rows - 1).end;  // (the last row of a tile sees most)
     const int kmin = paged_row_of(p, sq, hk, r0).end;
-    const int per = ((kend + p.nsplit - 1) / p.nsplit + 127) / 128 * 128;
-    const int k_lo = min(kend, split * per), k_hi = min(kend, k_lo + per);
+    int k_lo, k_hi;
+    paged_split(p, kend, split, k_lo, k_hi);
+    float *part = p.nsplit > 1 ? p.part + (((long)x * p.kv.n_kv + hk) * p.nsplit + split) * M * LD : nullptr;
+    if (part && k_lo >= k_hi) {  // a split that this sequence does not need
+        if ((int)threadIdx.x < rows) part[(long)threadIdx.x * LD + D] = -INFINITY, part[(long)threadIdx.x * LD + D + 1] = 0.f;
+        return;
+    }
     if (threadIdx.x == 0) s_bad[0] = 0;
 
     bf16x8 qf[CD][NP];
@@ -445,19 +507,23 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
 
     const char *kpool = (const char *)p.kv.k + hk * p.kv.head_stride * ES;
     const char *vpool = (const char *)p.kv.v + hk * p.kv.head_stride * ES + r16 * EV * ES;
+    // The next tile's entries of the table, one key a lane (past the end: the last key's, unused).
+    // Every load of the loop is made on every pass, so that each wait counts exactly the loads
+    // that it needs; keys that are none read page 0, slot 0, over and over the same row.
     const int key_of = lane & 31;
-    int page = -1, slot = 0;
-    auto entry = [&](int t0) {  // the table's entry of this lane's key
-        const int t = t0 + key_of;
-        page = -1;
-        if (t < k_hi) page = paged_page(p, b, t, slot);
+    int page = 0, slot = 0;
+    bool in = false;
+    auto entry = [&](int t0) {
+        in = t0 + key_of < k_hi;
+        page = paged_entry(p, b, max(0, min(t0 + key_of, k_hi - 1)), slot);
     };
     unsigned valid = 0;  // keys of the tile in flight that have a page
     float ks = 0.f, vs = 0.f;
     auto place = [&]() {
-        valid = (unsigned)__builtin_amdgcn_ballot_w64(page >= 0);
-        const long pg = max(page, 0), sl = page >= 0 ? slot : 0;
-        if (lane < 32) s_off[w][lane] = (pg * p.kv.page_stride + sl * p.kv.tok_stride) * ES;
+        in = in & (page >= 0) & (page < p.kv.n_pages);
+        valid = (unsigned)__builtin_amdgcn_ballot_w64(in);
+        const long pg = in ? page : 0, sl = in ? slot : 0;
+        s_off[w][lane & 31] = (pg * p.kv.page_stride + sl * p.kv.tok_stride) * ES;  // (both halves alike)
         if (EIGHT) {
             const long sc = (pg * p.kv.n_kv + hk) * p.kv.page_size + sl;
             ks = p.kv.ks[sc], vs = p.kv.vs[sc];
@@ -468,11 +534,11 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
     uint32_t kr[2][CD][KO::RW], vr[8][VO::RW];
     auto kload = [&]() {
 #pragma unroll
-        for (int a = 0; a < 2; ++a) KO::load(kpool + s_off[w][16 * a + r16], g, kr[a]);
+        for (int a = 0; a < 2; ++a) KO::template load<true>(kpool + s_off[w][16 * a + r16], g, kr[a]);
     };
     auto vload = [&]() {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) VO::load(vpool + s_off[w][4 * g + j + (j < 4 ? 0 : 12)], vr[j]);
+        for (int j = 0; j < 8; ++j) VO::template load<true>(vpool + s_off[w][4 * g + j + (j < 4 ? 0 : 12)], vr[j]);
     };
 
     floatx4 oacc[EV];
@@ -485,9 +551,12 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
     if (t0 < k_hi) {
         entry(t0);
         place();
-        kload();
-        vload();
         entry(t0 + 128);
+        __builtin_amdgcn_sched_barrier(0);  // (the same order as in the loop)
+        kload();
+        __builtin_amdgcn_sched_barrier(0);
+        vload();
+        __builtin_amdgcn_sched_barrier(0);
     }
     for (; t0 < k_hi; t0 += 128) {
         const unsigned now = valid;
@@ -507,7 +576,7 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
         }
         float vsc[8];
         if (EIGHT) {
-            if (lane < 32) s_sc[w][0][lane] = ks, s_sc[w][1][lane] = vs;
+            s_sc[w][0][lane & 31] = ks, s_sc[w][1][lane & 31] = vs;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -518,20 +587,20 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
                 for (int r = 0; r < 4; ++r) vsc[4 * a + r] = v[r];
             }
         }
+        place();          // the next tile's offsets (this tile's V is still in flight)
+        entry(t0 + 256);  // (loads end in the order of their issue: before K, or the next place() waits for V)
+        __builtin_amdgcn_sched_barrier(0);
+        kload();
+        __builtin_amdgcn_sched_barrier(0);
         // values of keys without a page, or past the end, are none
         if (now != 0xffffffffu) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const bool in = now >> (4 * g + j + (j < 4 ? 0 : 12)) & 1;
+                const bool there = now >> (4 * g + j + (j < 4 ? 0 : 12)) & 1;
 #pragma unroll
-                for (int e = 0; e < VO::RW; ++e) vr[j][e] = in ? vr[j][e] : 0u;
-                if (EIGHT) vsc[j] = in ? vsc[j] : 0.f;
+                for (int e = 0; e < VO::RW; ++e) vr[j][e] = there ? vr[j][e] : 0u;
+                if (EIGHT) vsc[j] = there ? vsc[j] : 0.f;
             }
-        }
-        const bool more = t0 + 128 < k_hi;
-        if (more) {
-            place();  // the next tile's offsets (this tile's V is already in flight)
-            kload();
         }
 #pragma unroll
         for (int a = 0; a < 2; ++a) s[a] *= sl2;
@@ -572,10 +641,7 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
             for (int k = 0; k < NK; ++k) vf[k] = as_bf16x8(pl[k]);
             oacc[i] = mfma_planes(vf, pf, oacc[i]);
         }
-        if (more) {
-            vload();
-            entry(t0 + 256);
-        }
+        vload();
     }
     // join the waves: means, so that sums near the end of fp32 stay in it
     l = paged_sum_rows(l);
@@ -593,7 +659,6 @@ __global__ void __launch_bounds__(256) paged_stream_kernel(const PagedAttnArgs p
 #pragma unroll
         for (int i = 0; i < EV; ++i) s_o[w][r16][(4 * g + r) * EV + i] = oacc[i][r] * f;
     __syncthreads();
-    float *part = p.nsplit > 1 ? p.part + (((long)x * p.kv.n_kv + hk) * p.nsplit + split) * M * LD : nullptr;
     float v[M * D / 256];
 #pragma unroll
     for (int k = 0; k < M * D / 256; ++k) {
@@ -645,13 +710,18 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x % p.kv.n_kv, rest = blockIdx.x / p.kv.n_kv, split = rest % p.nsplit, x = rest / p.nsplit;
     int b;
-    const int tile = paged_tile<M>(p, x, b);
-    const PagedSeq sq = paged_seq(p, b);
+    PagedSeq sq;
+    const int tile = p.sorted ? paged_tile_sorted<M>(p, x, b, sq) : paged_tile<M>(p, x, b, sq);
     const int r0 = tile * M, rows = min(M, sq.rows * p.G - r0);
     if (tile < 0 || rows <= 0) return;
     const int kend = paged_row_of(p, sq, hk, r0 + rows - 1).end;  // (the last row of a tile sees most)
-    const int per = ((kend + p.nsplit - 1) / p.nsplit + 63) / 64 * 64;
-    const int k_lo = min(kend, split * per), k_hi = min(kend, k_lo + per);
+    int k_lo, k_hi;
+    paged_split(p, kend, split, k_lo, k_hi);
+    float *part = p.nsplit > 1 ? p.part + (((long)x * p.kv.n_kv + hk) * p.nsplit + split) * M * LD : nullptr;
+    if (part && k_lo >= k_hi) {  // a split that this sequence does not need
+        if (tid < rows) part[(long)tid * LD + D] = -INFINITY, part[(long)tid * LD + D + 1] = 0.f;
+        return;
+    }
     if (tid < 4) s_bad[tid] = 0;
 
     // this wave's rows: 16 a block, and what its first and last see
@@ -672,19 +742,20 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
     const char *vpool = (const char *)p.kv.v + hk * p.kv.head_stride * ES + r16 * EV * ES;
     const int kj = NJ == 2 ? w & 1 : w;  // this wave's block of keys
     // the tile two ahead: its entries of the table (wave 0, one key a lane); one ahead: its places
-    int page = -1, slot = 0;
+    int page = 0, slot = 0;
+    bool in = false;
     float ks = 0.f, vs = 0.f;
     auto entry = [&](int t0) {
-        if (w == 0) {
-            const int t = t0 + lane;
-            page = -1;
-            if (lane < BK && t < k_hi) page = paged_page(p, b, t, slot);
+        if (w == 0) {  // (past the end: the last key's, unused)
+            in = lane < BK && t0 + lane < k_hi;
+            page = paged_entry(p, b, max(0, min(t0 + lane, k_hi - 1)), slot);
         }
     };
     auto place = [&](int at) {
         if (w == 0) {
-            const unsigned long long valid = __builtin_amdgcn_ballot_w64(page >= 0);
-            const long pg = max(page, 0), sl = page >= 0 ? slot : 0;
+            in = in & (page >= 0) & (page < p.kv.n_pages);
+            const unsigned long long valid = __builtin_amdgcn_ballot_w64(in);
+            const long pg = in ? page : 0, sl = in ? slot : 0;
             s_off[at][lane] = (pg * p.kv.page_stride + sl * p.kv.tok_stride) * ES;
             if (lane == 0) s_valid[at] = valid;
             if (EIGHT) {
@@ -852,7 +923,6 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
             }
     }
 
-    float *part = p.nsplit > 1 ? p.part + (((long)x * p.kv.n_kv + hk) * p.nsplit + split) * M * LD : nullptr;
 #pragma unroll
     for (int a = 0; a < NQ; ++a) {
         const int r = wr + 16 * a + r16;
@@ -903,37 +973,51 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
     if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) paged_again<D, CK, T>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
 }
 
-// Joins the splits of a tile's rows: one workgroup a (tile, key head)
+// Joins the splits of a tile's rows, one wave a row: lane i weighs split i (nsplit <= 64), then the
+// wave adds the means of the splits that have weight, sixteen in flight.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs p, int M)
 {
-    constexpr int LD = D + 4, PER = 256 / D * 1;
-    const int hk = blockIdx.x % p.kv.n_kv, x = blockIdx.x / p.kv.n_kv;
+    constexpr int LD = D + 4, E = (D + 63) / 64;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = blockIdx.x % (M / 4), rest = blockIdx.x / (M / 4), hk = rest % p.kv.n_kv, x = rest / p.kv.n_kv;
     int b;
-    const int tile = M == 16 ? paged_tile<16>(p, x, b) : M == 64 ? paged_tile<64>(p, x, b) : paged_tile<128>(p, x, b);
-    const PagedSeq sq = paged_seq(p, b);
-    const int r0 = tile * M, rows = min(M, sq.rows * p.G - r0);
-    if (tile < 0) return;
-    const float *part = p.part + ((long)x * p.kv.n_kv + hk) * p.nsplit * M * LD;
-    const int d = threadIdx.x % D;
-    for (int r = threadIdx.x / D; r < rows; r += PER) {
-        float mm = -INFINITY;
-        for (int s = 0; s < p.nsplit; ++s) mm = fmaxf(mm, part[((long)s * M + r) * LD + D]);
-        const float base = mm == -INFINITY ? 0.f : mm;
-        float ll = 0.f, v = 0.f;
-        for (int s = 0; s < p.nsplit; ++s) {
-            const float *q = part + ((long)s * M + r) * LD;
-            ll += paged_exp2(q[D] - base) * q[D + 1];
+    PagedSeq sq;
+    const int tile = M == 16 ? paged_tile<16>(p, x, b, sq) : M == 64 ? paged_tile<64>(p, x, b, sq) : paged_tile<128>(p, x, b, sq);
+    const int r = quarter * 4 + w;
+    if (tile < 0 || r >= sq.rows * p.G - tile * M) return;
+    const float *part = p.part + (((long)x * p.kv.n_kv + hk) * p.nsplit * M + r) * LD;
+    const long step = (long)M * LD;  // from a split to the next
+    const bool in = lane < p.nsplit;
+    const float m = in ? part[lane * step + D] : -INFINITY, l = in ? part[lane * step + D + 1] : 0.f;
+    const float mm = wave_max(m), base = mm == -INFINITY ? 0.f : mm;
+    float wt = l != 0.f ? paged_exp2(m - base) * l : 0.f;
+    const float ll = wave_sum(wt);
+    wt *= ll != 0.f ? 1.0f / ll : 0.f;
+    unsigned long long left = __builtin_amdgcn_ballot_w64(wt != 0.f);  // (a NaN weight too)
+    const int d = lane * E;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+    while (left) {
+        float f[16], q[16][E];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int s = left ? __builtin_ctzll(left) : 0;
+            f[k] = left ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), s)) : 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[k][e] = left && d < D ? part[s * step + d + e] : 0.f;
+            left &= left - 1;
         }
-        const float inv = ll != 0.f ? 1.0f / ll : 0.f;
-        for (int s = 0; s < p.nsplit; ++s) {
-            const float *q = part + ((long)s * M + r) * LD;
-            const float wt = paged_exp2(q[D] - base) * q[D + 1] * inv;
-            if (wt != 0.f) v = __builtin_fmaf(wt, q[d], v);
-        }
-        const PagedRow o = paged_row_of(p, sq, hk, r0 + r);
-        paged_put((T *)p.o + o.tok * p.o_st + o.h * p.o_sh + d, v);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = __builtin_fmaf(f[k], q[k][e], v[e]);
     }
+    if (d >= D) return;
+    const PagedRow o = paged_row_of(p, sq, hk, tile * M + r);
+#pragma unroll
+    for (int e = 0; e < E; ++e) paged_put((T *)p.o + o.tok * p.o_st + o.h * p.o_sh + d + e, v[e]);
 }
 
 template <int D, int CK, typename T>
@@ -943,7 +1027,7 @@ void paged_launch_as(const PagedAttnArgs &p, int rows, hipStream_t s)
     if (rows == 16) hipLaunchKernelGGL((paged_stream_kernel<D, CK, T>), grid, block, 0, s, p);
     else if (rows == 64) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1>), grid, block, 0, s, p);
     else if constexpr (sizeof(T) == 2 || D < 128) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 2>), grid, block, 0, s, p);
-    if (p.nsplit > 1) hipLaunchKernelGGL((paged_merge_kernel<D, T>), dim3((unsigned)p.tiles * p.kv.n_kv), block, 0, s, p, rows);
+    if (p.nsplit > 1) hipLaunchKernelGGL((paged_merge_kernel<D, T>), dim3((unsigned)p.tiles * p.kv.n_kv * (rows / 4)), block, 0, s, p, rows);
 }
 
 template <int D>
