@@ -5,10 +5,22 @@
 // 62 bits: 46 at 50257 logits), so sums are exact in any order and a threshold found by adding
 // bins is the one found by adding values one by one.  The order by falling value, lowest index first
 // among equals, is that of a whole-number key of the value; the kept set is always "keys above K,
-// and the first `ties` at K", so no row is sorted: K is found digit by digit from histograms of
-// counts (top-k) and of weights (top-p).
+// and the first `ties` at K".
+//
+// Three launches.  sample_max_kernel: the first maximum of each of C chunks of a row (C so that the
+// chip is full).  sample_hist_kernel: each chunk's histogram over bins of d = max - x, 64 to each
+// doubling of d, so that rows of any spread fit: of counts where top_k is small, of weights
+// otherwise.  sample_finish_kernel, a workgroup a row: the bins say where the cut falls; only that
+// bin's values are gathered from the row and sorted, the chunk that holds u follows from the
+// chunks' histograms, and only that chunk is walked.  Rows whose cut falls into a crowded bin
+// (thousands of values within 2 %), with top_k above 1024, or with an infinite maximum or
+// temperature take sample_row_general, which finds K digit by digit.
+//
+// Bound by the 64-bit exponentials of the weights (about 25 instructions of a logit) and the passes
+// over the logits, which stay in the caches after the first.
 #include "jas_common.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace jas {
@@ -21,6 +33,10 @@ struct SampleArgs {
     const int32_t *top_k;
     int32_t *ids;
     float *logp;
+    int C, chunk, vec;    // chunks of a row, logits of one; rows start on 16 bytes
+    uint32_t *chunk_key;  // [n][C] largest key of a chunk
+    int32_t *chunk_idx;   // and its first index
+    unsigned long long *hist;  // [n][C][NB]
 };
 
 // Keys grow with the value: -inf and NaN have the least, 0
@@ -62,7 +78,167 @@ __device__ __forceinline__ unsigned long long sample_mass(const SampleScale &sc,
     return (unsigned long long)rint(sample_w(sc, key) * sc.unit);
 }
 
-constexpr int ST = 1024;  // threads of a row
+constexpr int ST = 1024;      // threads of a row
+constexpr int NB = 1536;      // bins
+constexpr int SMALL_K = 1024; // largest top_k whose kept logits are sorted whole
+constexpr int CAP = 4096;     // logits that a row's cut may gather
+constexpr int MAX_CHUNKS = 1024;
+
+// Bin of d = max - x >= 0: below 2^-6 the first, then 64 to a doubling, the last from 2^17.9 up.
+// It does not fall as x falls.
+__device__ __forceinline__ int sample_bin(float d)
+{
+    const int t = (int)(__float_as_uint(fmaxf(d, 0x1p-7f)) >> 17) - (int)(0x3c800000u >> 17) + 1;
+    return max(0, min(t, NB - 1));
+}
+
+// Weight 2^shift e^((x - max) / T) as a whole number: c = log2(e) / T; 2^f by its series, |f| <= 1/2
+// (to 2^-47), and rounded by an addition of 2^52 (shift <= 51)
+__device__ __forceinline__ unsigned long long sample_weight(float x, double mx, double c, int shift)
+{
+    const double y = fmax(((double)x - mx) * c, -2000.0), n = rint(y), f = y - n;
+    double r = 4.4455382718708116e-10;  // ln(2)^k / k!, k = 11 .. 0
+    r = fma(r, f, 7.054911620801123e-09);
+    r = fma(r, f, 1.01780860092397e-07);
+    r = fma(r, f, 1.321548679014431e-06);
+    r = fma(r, f, 1.5252733804059841e-05);
+    r = fma(r, f, 0.0001540353039338161);
+    r = fma(r, f, 0.0013333558146428443);
+    r = fma(r, f, 0.009618129107628477);
+    r = fma(r, f, 0.05550410866482158);
+    r = fma(r, f, 0.24022650695910072);
+    r = fma(r, f, 0.6931471805599453);
+    r = fma(r, f, 1.0);
+    const double v = ldexp(r, (int)n + shift) + 0x1p52;
+    return (unsigned long long)__double_as_longlong(v) & 0xfffffffffffffull;
+}
+
+// How a row is drawn
+struct SampleRow {
+    float temp;
+    int top_k;      // 0: all
+    float top_p;    // 1: all
+    double min_p, u;
+    bool greedy, plain;  // the first maximum; 1 / T and the maximum are finite
+    double c;       // log2(e) / T
+};
+__device__ __forceinline__ SampleRow sample_row(const SampleArgs &p, int row, float mx)
+{
+    SampleRow r;
+    r.temp = p.temp ? p.temp[row] : 1.f;
+    r.top_k = p.top_k ? p.top_k[row] : 0;
+    if (r.top_k <= 0 || r.top_k >= p.V) r.top_k = 0;
+    r.greedy = !(r.temp > 0.f) || r.top_k == 1;
+    r.top_p = p.top_p ? p.top_p[row] : 1.f;
+    if (!(r.top_p < 1.f)) r.top_p = 1.f;
+    r.min_p = p.min_p && p.min_p[row] > 0.f ? fmin((double)p.min_p[row], 1.0) : 0.0;
+    const float u = p.u[row];
+    r.u = !(u > 0.f) ? 0.f : fminf(u, 0x1.fffffep-1f);
+    r.c = 1.4426950408889634074 / (double)r.temp;
+    r.plain = r.c > 0.0 && r.c < 1e300 && fabsf(mx) <= 3.402823466e38f;
+    return r;
+}
+
+// Calls f(x, index) for logits [i0, i1) of a row, by NT threads, each with rising indexes; i0 is a
+// multiple of 8.  CLEAN: a NaN as -inf.
+template <typename T, int NT, bool CLEAN = true, typename F>
+__device__ __forceinline__ void each_logit(const T *x, int i0, int i1, bool vec, F f)
+{
+    constexpr int E = 16 / sizeof(T), U = 8;
+    const auto clean = [](float v) { return CLEAN ? fmaxf(v, -INFINITY) : v; };
+    int i = i0;
+    if (vec) {  // eight loads in flight
+        const int whole = i0 + (i1 - i0) / E * E;
+        for (int at0 = i0 + (int)threadIdx.x * E; at0 < whole; at0 += U * NT * E) {
+            u32x4 v[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) v[k] = *(const u32x4 *)(x + min(at0 + k * NT * E, whole - E));
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int at = at0 + k * NT * E;
+                if (at >= whole) break;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (sizeof(T) == 4) f(clean(__uint_as_float(v[k][e])), at + e);
+                    else {
+                        f(clean(__uint_as_float(v[k][e] << 16)), at + 2 * e);
+                        f(clean(__uint_as_float(v[k][e] & 0xffff0000u)), at + 2 * e + 1);
+                    }
+                }
+            }
+        }
+        i = whole;
+    }
+    for (int at = i + (int)threadIdx.x; at < i1; at += NT) {
+        float v;
+        if constexpr (sizeof(T) == 4) v = x[at];
+        else v = bf16_to_f32(x[at]);
+        f(clean(v), at);
+    }
+}
+
+__device__ __forceinline__ void key_combine(uint32_t &k, int &i, uint32_t ok, int oi)
+{
+    if (ok > k || (ok == k && oi < i)) k = ok, i = oi;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) sample_max_kernel(const SampleArgs p)
+{
+    __shared__ uint32_t sk[4];
+    __shared__ int si[4];
+    const int row = blockIdx.y, c = blockIdx.x;
+    const T *x = (const T *)p.x + (long)row * p.ld;
+    float best = -INFINITY;
+    int i = 0x7fffffff;  // (a thread's indexes rise: a later equal is not larger, and neither is a NaN)
+    each_logit<T, 256, false>(x, c * p.chunk, min(p.V, (c + 1) * p.chunk), p.vec, [&](float v, int at) {
+        const bool more = v > best;
+        best = more ? v : best, i = more ? at : i;
+    });
+    uint32_t k = sample_key(best);
+    for (int o = 32; o; o >>= 1) key_combine(k, i, (uint32_t)__shfl_xor((int)k, o, WAVE), __shfl_xor(i, o, WAVE));
+    if ((threadIdx.x & 63) == 0) sk[threadIdx.x >> 6] = k, si[threadIdx.x >> 6] = i;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 4; ++w) key_combine(k, i, sk[w], si[w]);
+        p.chunk_key[(long)row * p.C + c] = k;
+        p.chunk_idx[(long)row * p.C + c] = i;
+    }
+}
+
+// The row's first maximum from its chunks', by every wave for itself
+__device__ __forceinline__ void row_max_key(const SampleArgs &p, int row, uint32_t &k, int &i)
+{
+    k = 0, i = 0x7fffffff;
+    for (int c = threadIdx.x & 63; c < p.C; c += 64) key_combine(k, i, p.chunk_key[(long)row * p.C + c], p.chunk_idx[(long)row * p.C + c]);
+    for (int o = 32; o; o >>= 1) key_combine(k, i, (uint32_t)__shfl_xor((int)k, o, WAVE), __shfl_xor(i, o, WAVE));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) sample_hist_kernel(const SampleArgs p)
+{
+    __shared__ unsigned long long bins[NB];
+    const int row = blockIdx.y, c = blockIdx.x;
+    uint32_t kmax;
+    int imax;
+    row_max_key(p, row, kmax, imax);
+    if (kmax == 0u) return;
+    const float mx = key_value(kmax);
+    const SampleRow r = sample_row(p, row, mx);
+    if (r.greedy || !r.plain || r.top_k > SMALL_K) return;
+    for (int b = threadIdx.x; b < NB; b += 256) bins[b] = 0;
+    __syncthreads();
+    const T *x = (const T *)p.x + (long)row * p.ld;
+    const int i0 = c * p.chunk, i1 = min(p.V, (c + 1) * p.chunk);
+    if (r.top_k) each_logit<T, 256>(x, i0, i1, p.vec, [&](float v, int) { atomicAdd((unsigned *)&bins[sample_bin(mx - v)], 1u); });
+    else each_logit<T, 256>(x, i0, i1, p.vec, [&](float v, int) {
+        const unsigned long long w = sample_weight(v, mx, r.c, p.shift);
+        if (w) atomicAdd(&bins[sample_bin(mx - v)], w);
+    });
+    __syncthreads();
+    unsigned long long *out = p.hist + ((long)row * p.C + c) * NB;
+    for (int b = threadIdx.x; b < NB; b += 256) out[b] = bins[b];
+}
 
 // first of the ST threads' 64-bit sums in thread order: exclusive prefix and total
 __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long *red, unsigned long long &total)
@@ -85,15 +261,17 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
     return before + inc - v;
 }
 
+// A row by one workgroup, whatever it holds: K by four passes of eight bits over the keys, each for
+// top-k and top-p
 template <typename T>
-__global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p)
+__device__ __attribute__((noinline)) void sample_row_general(const SampleArgs &p, int row, unsigned long long *red)
 {
     __shared__ unsigned cnt[256];
-    __shared__ unsigned long long mass[256], red[ST / 64];
+    __shared__ unsigned long long mass[256];
     __shared__ unsigned s_key, s_ties;
     __shared__ unsigned long long s_mass;
     __shared__ float s_max[16];
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63;
     const T *x = (const T *)p.x + (long)row * p.ld;
     const int V = p.V;
     uint32_t kmax = 0;
@@ -263,13 +441,369 @@ __global__ void __launch_bounds__(ST) sample_kernel(const SampleArgs p)
     }
 }
 
+// Sorts the n <= CAP different entries of s to fall, by the whole workgroup: few by counting the
+// larger ones of each, more by bitonic exchanges (s has room for the next power of two)
+__device__ __forceinline__ void sort_falling(unsigned long long *s, int n)
+{
+    if (n <= 256) {
+        const int i = threadIdx.x;
+        const unsigned long long e = i < n ? s[i] : 0;
+        int rank = 0;
+        if (i < (n + 63) / 64 * 64)
+            for (int j = 0; j < n; ++j) rank += s[j] > e;
+        __syncthreads();
+        if (i < n) s[rank] = e;
+        __syncthreads();
+        return;
+    }
+    const int m = 1 << (32 - __builtin_clz(n - 1));
+    for (int i = n + threadIdx.x; i < m; i += ST) s[i] = 0;
+    for (int k = 2; k <= m; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < m / 2; i += ST) {
+                const int a = 2 * i - (i & (j - 1)), b = a + j;
+                const unsigned long long u = s[a], v = s[b];
+                if ((u < v) == ((a & k) == 0)) s[a] = v, s[b] = u;
+            }
+        }
+    __syncthreads();
+}
+
+// Entries of a list of logits: key and index, falling by key, then rising by index
+__device__ __forceinline__ unsigned long long list_entry(uint32_t key, int i) { return (unsigned long long)key << 32 | (uint32_t)~i; }
+__device__ __forceinline__ uint32_t entry_key(unsigned long long e) { return (uint32_t)(e >> 32); }
+__device__ __forceinline__ int entry_index(unsigned long long e) { return (int)~(uint32_t)e; }
+
+struct FinishShared {
+    unsigned long long list[CAP];
+    unsigned long long sums[NB];
+    unsigned long long red[ST / 64], wave_sum[ST / 64], sum[2];
+    unsigned tie[MAX_CHUNKS], wave_ties[ST / 64];
+    unsigned n, key_lo, key_hi;
+    int at[4];
+};
+static_assert(NB >= ST && NB <= 2 * ST && MAX_CHUNKS <= ST, "a bin or two, and a chunk, a thread");
+
+// False: the row is one for sample_row_general
+template <typename T>
+__device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, FinishShared &sh)
+{
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const T *x = (const T *)p.x + (long)row * p.ld;
+    uint32_t kmax;
+    int imax;
+    row_max_key(p, row, kmax, imax);
+    if (kmax == 0u) {  // nothing above -inf
+        if (tid == 0) {
+            p.ids[row] = -1;
+            if (p.logp) p.logp[row] = -INFINITY;
+        }
+        return true;
+    }
+    const float mx = key_value(kmax);
+    const SampleRow r = sample_row(p, row, mx);
+    if (r.greedy) {
+        if (tid == 0) {
+            p.ids[row] = imax;
+            if (p.logp) p.logp[row] = 0.f;
+        }
+        return true;
+    }
+    if (!r.plain || r.top_k > SMALL_K) return false;
+    const SampleScale sc = {(double)mx, (double)r.temp, ldexp(1.0, p.shift), false};
+    const unsigned long long *hist = p.hist + (long)row * p.C * NB;
+    auto logit = [&](int i) {
+        float v;
+        if constexpr (sizeof(T) == 4) v = x[i];
+        else v = bf16_to_f32(x[i]);
+        return fmaxf(v, -INFINITY);
+    };
+    // the logits of bins lo .. hi, in any order (false: too many)
+    int n = 0;
+    auto gather = [&](int lo, int hi) {
+        __syncthreads();
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        each_logit<T, ST>(x, 0, p.V, p.vec, [&](float v, int at) {
+            const int b = sample_bin(mx - v);
+            if (b >= lo && b <= hi && v > -INFINITY) {
+                const unsigned k = atomicAdd(&sh.n, 1u);
+                if (k < CAP) sh.list[k] = list_entry(sample_key(v), at);
+            }
+        });
+        __syncthreads();
+        n = (int)sh.n;
+        return n <= CAP;
+    };
+    // the chunks' bins together, and the bin where their sum reaches what is wanted
+    unsigned long long total = 0;
+    for (int b = tid; b < NB; b += ST) {
+        unsigned long long t = 0;
+        int c = 0;
+        for (; c + 8 <= p.C; c += 8) {
+            unsigned long long h[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) h[k] = hist[(long)(c + k) * NB + b];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t += h[k];
+        }
+        for (; c < p.C; ++c) t += hist[(long)c * NB + b];
+        sh.sums[b] = t;
+    }
+    if (tid == 0) sh.at[0] = -1;
+    __syncthreads();
+    {
+        const unsigned long long a = 2 * tid < NB ? sh.sums[2 * tid] : 0, b = 2 * tid + 1 < NB ? sh.sums[2 * tid + 1] : 0;
+        const unsigned long long before = block_scan(a + b, sh.red, total);
+        const double want = r.top_k ? (double)r.top_k : (double)r.top_p * (double)total;
+        if (r.top_k || r.top_p < 1.f) {  // (one thread finds it)
+            if (a && ((double)before < want || before == 0) && (double)(before + a) >= want) sh.at[0] = 2 * tid, sh.sum[0] = before;
+            else if (b && ((double)(before + a) < want || before + a == 0) && (double)(before + a + b) >= want) sh.at[0] = 2 * tid + 1, sh.sum[0] = before + a;
+        }
+        __syncthreads();
+    }
+    if (r.top_k) {  // few: all that top-k keeps, in LDS
+        // (fewer logits above -inf than top_k: all of them)
+        if (!gather(0, sh.at[0] < 0 ? NB - 1 : sh.at[0])) return false;
+        sort_falling(sh.list, n);
+        const int kept = min(n, r.top_k);
+        const unsigned long long e = tid < kept ? sh.list[tid] : 0;
+        const float v = key_value(entry_key(e));
+        unsigned long long wt = tid < kept ? sample_weight(v, mx, r.c, p.shift) : 0, all;
+        const unsigned long long before = block_scan(wt, sh.red, all);
+        if (r.top_p < 1.f && tid > 0 && !((double)before < (double)r.top_p * (double)all)) wt = 0;
+        if (r.min_p > 0.0 && tid < kept && !(exp(sample_z(sc, v)) >= r.min_p)) wt = 0;
+        // in index order
+        if (tid < kept) sh.list[tid] = (unsigned long long)(uint32_t)~entry_index(e) << 32 | (uint32_t)tid;
+        sh.sums[tid] = wt;
+        __syncthreads();
+        sort_falling(sh.list, kept);
+        const unsigned long long f = tid < kept ? sh.list[tid] : 0;
+        wt = tid < kept ? sh.sums[(uint32_t)f] : 0;
+        const unsigned long long upto = block_scan(wt, sh.red, all) + wt;
+        const double target = r.u * (double)all;
+        if (wt && (double)upto > target && !((double)(upto - wt) > target)) {
+            const int at = (int)~(uint32_t)(f >> 32);
+            p.ids[row] = at;
+            if (p.logp) p.logp[row] = (float)(sample_z(sc, logit(at)) - log((double)all / sc.unit));
+        }
+        return true;
+    }
+
+    // The cut: bins below lo are kept whole, those of lo .. hi logit by logit (keys above K, the first
+    // `ties` at K, weights of at least min_p), the rest not
+    int lo = NB, hi = NB - 1;
+    uint32_t K = 0;
+    unsigned ties = 0;
+    constexpr int PER = CAP / ST;
+    if (r.top_p < 1.f) {
+        lo = hi = sh.at[0];
+        unsigned long long above = sh.sum[0];
+        if (lo < 0 || !gather(lo, hi)) return false;
+        const double want = (double)r.top_p * (double)total;
+        // K: the gathered keys' range cut into 1024 parts until the part that reaches what is
+        // wanted holds one key
+        uint32_t key[PER];
+        unsigned long long wt[PER];
+        if (tid == 0) sh.key_lo = 0xffffffffu, sh.key_hi = 0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int i = tid + k * ST;
+            key[k] = i < n ? entry_key(sh.list[i]) : 0;
+            wt[k] = i < n ? sample_weight(key_value(key[k]), mx, r.c, p.shift) : 0;
+            if (i < n) atomicMin(&sh.key_lo, key[k]), atomicMax(&sh.key_hi, key[k]);
+        }
+        __syncthreads();
+        uint32_t klo = sh.key_lo, khi = sh.key_hi;
+        while (klo < khi) {
+            const int shift = max(0, 22 - __builtin_clz(khi - klo));  // (khi - klo) >> shift < 1024
+            sh.sums[tid] = 0;
+            if (tid == 0) sh.at[1] = -1;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (key[k] >= klo && key[k] <= khi) atomicAdd(&sh.sums[(khi - key[k]) >> shift], wt[k]);
+            __syncthreads();
+            const unsigned long long a = sh.sums[tid];
+            unsigned long long all;
+            const unsigned long long before = above + block_scan(a, sh.red, all);
+            if (a && ((double)before < want || before == 0) && (double)(before + a) >= want) sh.at[1] = tid, sh.sum[0] = before;
+            if (tid == 0) sh.key_lo = 0xffffffffu, sh.key_hi = 0;
+            __syncthreads();
+            const int part = sh.at[1];
+            if (part < 0) return false;  // (none: weights that all round to nothing)
+            above = sh.sum[0];
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (key[k] >= klo && key[k] <= khi && (int)((khi - key[k]) >> shift) == part) atomicMin(&sh.key_lo, key[k]), atomicMax(&sh.key_hi, key[k]);
+            __syncthreads();
+            klo = sh.key_lo, khi = sh.key_hi;
+            __syncthreads();
+        }
+        K = klo;
+        // of K's equals, as many as start below what is wanted; one at least where nothing lies above
+        const unsigned long long each = sample_weight(key_value(K), mx, r.c, p.shift);
+        const double q = each ? ceil((want - (double)above) / (double)each) : 0.0;
+        ties = q < 1.0 ? 0u : q > (double)p.V ? (unsigned)p.V : (unsigned)q;
+        while (ties && !((double)(above + (ties - 1) * each) < want)) --ties;
+        while (each && ties < (unsigned)p.V && (double)(above + ties * each) < want) ++ties;
+        if (ties == 0 && above == 0) ties = 1;
+    }
+    int mlo = NB;  // from this bin on weights are compared with min_p
+    if (r.min_p > 0.0) {
+        const double d = -(double)r.temp * log(r.min_p);
+        mlo = max(0, sample_bin((float)(d * (1 - 0x1p-20))) - 1);
+        const int mhi = min(sample_bin((float)(d * (1 + 0x1p-20))) + 1, NB - 1);
+        const int nlo = min(lo, mlo), nhi = min(hi, mhi);
+        if (nlo != lo || nhi != hi) {
+            lo = nlo, hi = nhi;
+            if (!gather(lo, hi)) return false;
+        }
+    }
+    const auto heavy = [&](float v, int bin) { return !(r.min_p > 0.0 && bin >= mlo) || exp(sample_z(sc, v)) >= r.min_p; };
+    // what each chunk keeps: its bins below the cut, the cut's keys above K, and its share of the ties
+    __syncthreads();
+    for (int c = w; c < p.C; c += ST / 64) {
+        unsigned long long t = 0;
+        for (int b = lane; b < lo; b += 64) t += hist[(long)c * NB + b];
+        for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o, WAVE);
+        if (lane == 0) sh.sums[c] = t, sh.tie[c] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += ST) {
+        const unsigned long long e = sh.list[i];
+        const uint32_t key = entry_key(e);
+        const float v = key_value(key);
+        const int c = entry_index(e) / p.chunk;
+        if (key < K || !heavy(v, sample_bin(mx - v))) continue;
+        if (key == K) atomicAdd(&sh.tie[c], 1u);
+        else atomicAdd(&sh.sums[c], sample_weight(v, mx, r.c, p.shift));
+    }
+    __syncthreads();
+    unsigned long long mine = 0, tied;
+    {
+        const unsigned t = tid < p.C ? sh.tie[tid] : 0;
+        const unsigned long long before = block_scan(t, sh.red, tied);
+        if (tid < p.C) {
+            mine = sh.sums[tid];
+            if (t && before < ties) mine += (unsigned long long)min(t, ties - (unsigned)before) * sample_weight(key_value(K), mx, r.c, p.shift);
+            sh.tie[tid] = (unsigned)before;
+        }
+    }
+    const unsigned long long start = block_scan(mine, sh.red, total);
+    const double target = r.u * (double)total;
+    if (mine && !((double)start > target) && (double)(start + mine) > target) sh.at[3] = tid, sh.sum[1] = start;
+    __syncthreads();
+    // that chunk's logits in 16 stretches, a wave each: what they keep, then the one with the target
+    const int c0 = sh.at[3] * p.chunk, c1 = min(p.V, c0 + p.chunk);
+    const int per = ((c1 - c0 + ST / 64 - 1) / (ST / 64) + 63) / 64 * 64;
+    const int i0 = min(c1, c0 + w * per), i1 = min(c1, i0 + per);
+    // a logit's weight if it is kept, or whether it is one of K's equals that count
+    auto weigh = [&](float v, bool &tie) {
+        const uint32_t key = sample_key(v);
+        const int bin = sample_bin(mx - v);
+        const bool in = key && (bin < lo || (bin <= hi && key >= K && heavy(v, bin)));
+        tie = in && K && key == K;
+        return in && !tie ? sample_weight(v, mx, r.c, p.shift) : 0ull;
+    };
+    constexpr int U = 8;  // loads in flight
+    float v[U];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int at = i + 64 * k + lane;
+            v[k] = logit(min(at, p.V - 1));
+            if (at >= i1) v[k] = -INFINITY;
+        }
+    };
+    unsigned long long m = 0;
+    unsigned t = 0;
+    for (int i = i0; i < i1; i += 64 * U) {
+        fetch(i);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            bool tie;
+            m += weigh(v[k], tie);
+            t += tie;
+        }
+    }
+    for (int o = 32; o; o >>= 1) m += __shfl_xor(m, o, WAVE), t += __shfl_xor(t, o, WAVE);
+    if (lane == 0) sh.wave_sum[w] = m, sh.wave_ties[w] = t;
+    __syncthreads();
+    const unsigned long long each = K ? sample_weight(key_value(K), mx, r.c, p.shift) : 0;
+    unsigned long long run = sh.sum[1];
+    unsigned seen = sh.tie[sh.at[3]];  // K's equals before this stretch
+    for (int k = 0; k <= w; ++k) {
+        const unsigned long long kept = sh.wave_sum[k] + (seen < ties ? min(sh.wave_ties[k], ties - seen) : 0) * each;
+        if (k == w) m = kept;
+        else run += kept, seen += sh.wave_ties[k];
+    }
+    if (!m || (double)run > target || !((double)(run + m) > target)) return true;
+    for (int i = i0; i < i1; i += 64 * U) {  // one wave is left
+        fetch(i);
+#pragma unroll 1
+        for (int k = 0; k < U; ++k) {
+            float vk = v[0];
+#pragma unroll
+            for (int q = 1; q < U; ++q) vk = k == q ? v[q] : vk;
+            bool tie;
+            unsigned long long wt = weigh(vk, tie);
+            const unsigned long long eq = __builtin_amdgcn_ballot_w64(tie);
+            if (tie && seen + __popcll(eq & ((1ull << lane) - 1)) < ties) wt = each;
+            seen += __popcll(eq);
+            unsigned long long inc = wt;
+            for (int o = 1; o < 64; o <<= 1) {
+                const unsigned long long below = __shfl_up(inc, o, WAVE);
+                if (lane >= o) inc += below;
+            }
+            const unsigned long long hit = __builtin_amdgcn_ballot_w64(wt && (double)(run + inc) > target);
+            if (hit) {
+                if (lane == __ffsll((long long)hit) - 1) {
+                    p.ids[row] = i + 64 * k + lane;
+                    if (p.logp) p.logp[row] = (float)(sample_z(sc, vk) - log((double)total / sc.unit));
+                }
+                return true;
+            }
+            run += __shfl(inc, 63, WAVE);
+        }
+    }
+    return true;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ST) sample_finish_kernel(const SampleArgs p)
+{
+    __shared__ FinishShared sh;
+    if (!sample_finish<T>(p, blockIdx.x, sh)) {
+        __syncthreads();
+        sample_row_general<T>(p, blockIdx.x, sh.red);
+    }
+}
+
 } // namespace jas
 
 using namespace jas;
 
+// Chunks of a row: of at least 4096 logits (a histogram of 12 KB each), until some 1024 workgroups
+// have one
+static void sample_chunks(int n, int V, int &C, int &chunk)
+{
+    C = std::max(1, std::min({(1024 + n - 1) / n, (V + 4095) / 4096, MAX_CHUNKS}));
+    chunk = ((V + C - 1) / C + 1023) / 1024 * 1024;
+    C = (V + chunk - 1) / chunk;
+}
+
 extern "C" {
 
-size_t jas_sample_workspace(int n, int V) { return 0; }
+size_t jas_sample_workspace(int n, int V)
+{
+    if (n <= 0 || V <= 0 || V > 1 << 22) return 0;
+    int C, chunk;
+    sample_chunks(n, V, C, chunk);
+    return (size_t)n * C * (NB * sizeof(unsigned long long) + 2 * sizeof(uint32_t));
+}
 
 jas_status jas_sample(const void *x, int n, int V, int64_t ld, const float *temp, const int32_t *top_k, const float *top_p,
                       const float *min_p, const float *u, int32_t *ids, float *logp, int dtype, void *work, jas_stream_t stream)
@@ -279,12 +813,29 @@ jas_status jas_sample(const void *x, int n, int V, int64_t ld, const float *temp
     JAS_CHECK(dtype == JAS_F32 || dtype == JAS_BF16, JAS_ERR_INVALID, "jas_sample: logits are JAS_F32 or JAS_BF16");
     JAS_CHECK((uintptr_t)x % (dtype == JAS_F32 ? 4 : 2) == 0, JAS_ERR_INVALID, "jas_sample: logits aligned to their elements");
     if (!n) return JAS_OK;
+    JAS_CHECK(n <= 65535, JAS_ERR_INVALID, "jas_sample: at most 65535 rows");
+    JAS_CHECK(work && (uintptr_t)work % 16 == 0, JAS_ERR_INVALID, "jas_sample: need a workspace aligned to 16 bytes");
     int bits = 0;
     while ((1 << bits) < V) ++bits;
-    SampleArgs p{x, n, V, std::min(52, 62 - bits), (long)ld, temp, top_p, min_p, u, top_k, ids, logp};
+    SampleArgs p{};
+    p.x = x, p.n = n, p.V = V, p.shift = std::min(51, 62 - bits), p.ld = (long)ld;
+    p.temp = temp, p.top_k = top_k, p.top_p = top_p, p.min_p = min_p, p.u = u, p.ids = ids, p.logp = logp;
+    sample_chunks(n, V, p.C, p.chunk);
+    p.vec = (uintptr_t)x % 16 == 0 && ld * (dtype == JAS_F32 ? 4 : 2) % 16 == 0;
+    p.hist = (unsigned long long *)work;
+    p.chunk_key = (uint32_t *)(p.hist + (size_t)n * p.C * NB);
+    p.chunk_idx = (int32_t *)(p.chunk_key + (size_t)n * p.C);
     hipStream_t s = stream_or_default(stream);
-    if (dtype == JAS_F32) hipLaunchKernelGGL(sample_kernel<float>, dim3(n), dim3(ST), 0, s, p);
-    else hipLaunchKernelGGL(sample_kernel<uint16_t>, dim3(n), dim3(ST), 0, s, p);
+    const dim3 grid(p.C, n);
+    if (dtype == JAS_F32) {
+        hipLaunchKernelGGL(sample_max_kernel<float>, grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL(sample_hist_kernel<float>, grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL(sample_finish_kernel<float>, dim3(n), dim3(ST), 0, s, p);
+    } else {
+        hipLaunchKernelGGL(sample_max_kernel<uint16_t>, grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL(sample_hist_kernel<uint16_t>, grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL(sample_finish_kernel<uint16_t>, dim3(n), dim3(ST), 0, s, p);
+    }
     JAS_LAUNCH_CHECK();
     return JAS_OK;
 }
