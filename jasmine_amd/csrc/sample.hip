@@ -33,7 +33,7 @@ struct SampleArgs {
     const int32_t *top_k;
     int32_t *ids;
     float *logp;
-    int C, chunk, vec;    // chunks of a row, logits of one; rows start on 16 bytes
+    int C, chunk, vec;    // chunks of a row, logits of one (a multiple of 1024); rows start on 16 bytes
     uint32_t *chunk_key;  // [n][C] largest key of a chunk
     int32_t *chunk_idx;   // and its first index
     unsigned long long *hist;  // [n][C][NB]
@@ -92,6 +92,12 @@ __device__ __forceinline__ int sample_bin(float d)
     return max(0, min(t, NB - 1));
 }
 
+// d from which bin b starts, for b up to NB (the last bin has no end)
+__device__ __forceinline__ float bin_edge(int b)
+{
+    return b <= 0 ? 0.f : b >= NB ? INFINITY : __uint_as_float((uint32_t)(b - 1 + (0x3c800000 >> 17)) << 17);
+}
+
 // Weight 2^shift e^((x - max) / T) as a whole number: c = log2(e) / T; 2^f by its series, |f| <= 1/2
 // (to 2^-47), and rounded by an addition of 2^52 (shift <= 51)
 __device__ __forceinline__ unsigned long long sample_weight(float x, double mx, double c, int shift)
@@ -139,42 +145,47 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs &p, int row, fl
     return r;
 }
 
-// Calls f(x, index) for logits [i0, i1) of a row, by NT threads, each with rising indexes; i0 is a
-// multiple of 8.  CLEAN: a NaN as -inf.
+// Logits of a row before the first on 16 bytes
+template <typename T>
+__device__ __forceinline__ int logits_before_16(const T *x)
+{
+    return (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T));
+}
+
+// Calls f(x, index) for logits [i0, i1) of a row, by NT threads, each with rising indexes.  CLEAN: a
+// NaN as -inf.
 template <typename T, int NT, bool CLEAN = true, typename F>
-__device__ __forceinline__ void each_logit(const T *x, int i0, int i1, bool vec, F f)
+__device__ __forceinline__ void each_logit(const T *x, int i0, int i1, F f)
 {
     constexpr int E = 16 / sizeof(T), U = 8;
     const auto clean = [](float v) { return CLEAN ? fmaxf(v, -INFINITY) : v; };
-    int i = i0;
-    if (vec) {  // eight loads in flight
-        const int whole = i0 + (i1 - i0) / E * E;
-        for (int at0 = i0 + (int)threadIdx.x * E; at0 < whole; at0 += U * NT * E) {
-            u32x4 v[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k) v[k] = *(const u32x4 *)(x + min(at0 + k * NT * E, whole - E));
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const int at = at0 + k * NT * E;
-                if (at >= whole) break;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (sizeof(T) == 4) f(clean(__uint_as_float(v[k][e])), at + e);
-                    else {
-                        f(clean(__uint_as_float(v[k][e] << 16)), at + 2 * e);
-                        f(clean(__uint_as_float(v[k][e] & 0xffff0000u)), at + 2 * e + 1);
-                    }
-                }
-            }
-        }
-        i = whole;
-    }
-    for (int at = i + (int)threadIdx.x; at < i1; at += NT) {
+    const auto one = [&](int at) {
         float v;
         if constexpr (sizeof(T) == 4) v = x[at];
         else v = bf16_to_f32(x[at]);
         f(clean(v), at);
+    };
+    const int head = min(i1, i0 + logits_before_16(x + i0)), whole = head + (i1 - head) / E * E;
+    if (i0 + (int)threadIdx.x < head) one(i0 + (int)threadIdx.x);
+    for (int at0 = head + (int)threadIdx.x * E; at0 < whole; at0 += U * NT * E) {  // eight loads in flight
+        u32x4 v[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) v[k] = *(const u32x4 *)(x + min(at0 + k * NT * E, whole - E));
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int at = at0 + k * NT * E;
+            if (at >= whole) break;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(T) == 4) f(clean(__uint_as_float(v[k][e])), at + e);
+                else {
+                    f(clean(__uint_as_float(v[k][e] << 16)), at + 2 * e);
+                    f(clean(__uint_as_float(v[k][e] & 0xffff0000u)), at + 2 * e + 1);
+                }
+            }
+        }
     }
+    if (whole + (int)threadIdx.x < i1) one(whole + (int)threadIdx.x);
 }
 
 __device__ __forceinline__ void key_combine(uint32_t &k, int &i, uint32_t ok, int oi)
@@ -191,7 +202,7 @@ __global__ void __launch_bounds__(256) sample_max_kernel(const SampleArgs p)
     const T *x = (const T *)p.x + (long)row * p.ld;
     float best = -INFINITY;
     int i = 0x7fffffff;  // (a thread's indexes rise: a later equal is not larger, and neither is a NaN)
-    each_logit<T, 256, false>(x, c * p.chunk, min(p.V, (c + 1) * p.chunk), p.vec, [&](float v, int at) {
+    each_logit<T, 256, false>(x, c * p.chunk, min(p.V, (c + 1) * p.chunk), [&](float v, int at) {
         const bool more = v > best;
         best = more ? v : best, i = more ? at : i;
     });
@@ -230,8 +241,8 @@ __global__ void __launch_bounds__(256) sample_hist_kernel(const SampleArgs p)
     __syncthreads();
     const T *x = (const T *)p.x + (long)row * p.ld;
     const int i0 = c * p.chunk, i1 = min(p.V, (c + 1) * p.chunk);
-    if (r.top_k) each_logit<T, 256>(x, i0, i1, p.vec, [&](float v, int) { atomicAdd((unsigned *)&bins[sample_bin(mx - v)], 1u); });
-    else each_logit<T, 256>(x, i0, i1, p.vec, [&](float v, int) {
+    if (r.top_k) each_logit<T, 256>(x, i0, i1, [&](float v, int) { atomicAdd((unsigned *)&bins[sample_bin(mx - v)], 1u); });
+    else each_logit<T, 256>(x, i0, i1, [&](float v, int) {
         const unsigned long long w = sample_weight(v, mx, r.c, p.shift);
         if (w) atomicAdd(&bins[sample_bin(mx - v)], w);
     });
@@ -478,9 +489,8 @@ __device__ __forceinline__ int entry_index(unsigned long long e) { return (int)~
 struct FinishShared {
     unsigned long long list[CAP];
     unsigned long long sums[NB];
-    unsigned long long red[ST / 64], wave_sum[ST / 64], sum[2];
-    unsigned tie[MAX_CHUNKS], wave_ties[ST / 64];
-    unsigned n, key_lo, key_hi;
+    unsigned long long red[ST / 64], sum[2];
+    unsigned tie[MAX_CHUNKS], n;
     int at[4];
 };
 static_assert(NB >= ST && NB <= 2 * ST && MAX_CHUNKS <= ST, "a bin or two, and a chunk, a thread");
@@ -519,19 +529,46 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
         else v = bf16_to_f32(x[i]);
         return fmaxf(v, -INFINITY);
     };
-    // the logits of bins lo .. hi, in any order (false: too many)
+    // The logits of bins lo .. hi, in any order (false: too many).  A thread marks its logits by two
+    // comparisons each (a little outside the bins' edges) and looks again at the few it marked.
     int n = 0;
     auto gather = [&](int lo, int hi) {
         __syncthreads();
         if (tid == 0) sh.n = 0;
         __syncthreads();
-        each_logit<T, ST>(x, 0, p.V, p.vec, [&](float v, int at) {
+        const float top = mx - bin_edge(lo) * (1 - 0x1p-20f), bottom = mx - bin_edge(hi + 1) * (1 + 0x1p-20f);
+        const float vtop = top + fabsf(top) * 0x1p-20f, vbottom = bottom - fabsf(bottom) * 0x1p-20f;
+        auto look = [&](int at) {
+            const float v = logit(at);
             const int b = sample_bin(mx - v);
             if (b >= lo && b <= hi && v > -INFINITY) {
                 const unsigned k = atomicAdd(&sh.n, 1u);
                 if (k < CAP) sh.list[k] = list_entry(sample_key(v), at);
             }
-        });
+        };
+        constexpr int E = 16 / sizeof(T), U = 32 / E;  // 32 logits a thread and batch
+        const int head = min(p.V, logits_before_16(x)), whole = head + (p.V - head) / E * E;
+        if (tid < head) look(tid);
+        for (int at0 = head + tid * E; at0 < whole; at0 += U * ST * E) {
+            u32x4 v[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) v[k] = *(const u32x4 *)(x + min(at0 + k * ST * E, whole - E));
+            unsigned marks = 0;
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    float f;
+                    if constexpr (sizeof(T) == 4) f = __uint_as_float(v[k][e]);
+                    else f = __uint_as_float(e % 2 ? v[k][e / 2] & 0xffff0000u : v[k][e / 2] << 16);
+                    marks |= (unsigned)(f >= vbottom && f <= vtop) << (k * E + e);
+                }
+            for (; marks; marks &= marks - 1) {
+                const int bit = __builtin_ctz(marks), at = at0 + bit / E * (ST * E) + bit % E;
+                if (at < whole) look(at);  // (past the end the last vector was read again)
+            }
+        }
+        if (whole + tid < p.V) look(whole + tid);
         __syncthreads();
         n = (int)sh.n;
         return n <= CAP;
@@ -540,15 +577,13 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
     unsigned long long total = 0;
     for (int b = tid; b < NB; b += ST) {
         unsigned long long t = 0;
-        int c = 0;
-        for (; c + 8 <= p.C; c += 8) {
+        for (int c = 0; c < p.C; c += 8) {
             unsigned long long h[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) h[k] = hist[(long)(c + k) * NB + b];
+            for (int k = 0; k < 8; ++k) h[k] = c + k < p.C ? hist[(long)(c + k) * NB + b] : 0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) t += h[k];
         }
-        for (; c < p.C; ++c) t += hist[(long)c * NB + b];
         sh.sums[b] = t;
     }
     if (tid == 0) sh.at[0] = -1;
@@ -602,47 +637,43 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
         unsigned long long above = sh.sum[0];
         if (lo < 0 || !gather(lo, hi)) return false;
         const double want = (double)r.top_p * (double)total;
-        // K: the gathered keys' range cut into 1024 parts until the part that reaches what is
-        // wanted holds one key
+        // K: the keys between the bin's edges cut into 1024 parts, then the part that reaches what
+        // is wanted, until a part is one key (bf16: of 16 bits)
+        constexpr int KS = sizeof(T) == 2 ? 16 : 0;
         uint32_t key[PER];
         unsigned long long wt[PER];
-        if (tid == 0) sh.key_lo = 0xffffffffu, sh.key_hi = 0;
-        __syncthreads();
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int i = tid + k * ST;
             key[k] = i < n ? entry_key(sh.list[i]) : 0;
             wt[k] = i < n ? sample_weight(key_value(key[k]), mx, r.c, p.shift) : 0;
-            if (i < n) atomicMin(&sh.key_lo, key[k]), atomicMax(&sh.key_hi, key[k]);
+            key[k] >>= KS;
         }
-        __syncthreads();
-        uint32_t klo = sh.key_lo, khi = sh.key_hi;
-        while (klo < khi) {
-            const int shift = max(0, 22 - __builtin_clz(khi - klo));  // (khi - klo) >> shift < 1024
+        const float top = mx - bin_edge(lo) * (1 - 0x1p-20f), bottom = lo == NB - 1 ? -3.402823466e38f : mx - bin_edge(lo + 1) * (1 + 0x1p-20f);
+        uint32_t khi = sample_key(top + fabsf(top) * 0x1p-20f) >> KS, klo = max(sample_key(bottom - fabsf(bottom) * 0x1p-20f) >> KS, 1u);
+        while (true) {
+            const int shift = klo == khi ? 0 : max(0, 22 - __builtin_clz(khi - klo));  // (khi - klo) >> shift < 1024
             sh.sums[tid] = 0;
             if (tid == 0) sh.at[1] = -1;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < PER; ++k)
-                if (key[k] >= klo && key[k] <= khi) atomicAdd(&sh.sums[(khi - key[k]) >> shift], wt[k]);
+                if (wt[k] && key[k] >= klo && key[k] <= khi) atomicAdd(&sh.sums[(khi - key[k]) >> shift], wt[k]);
             __syncthreads();
             const unsigned long long a = sh.sums[tid];
             unsigned long long all;
             const unsigned long long before = above + block_scan(a, sh.red, all);
             if (a && ((double)before < want || before == 0) && (double)(before + a) >= want) sh.at[1] = tid, sh.sum[0] = before;
-            if (tid == 0) sh.key_lo = 0xffffffffu, sh.key_hi = 0;
             __syncthreads();
             const int part = sh.at[1];
-            if (part < 0) return false;  // (none: weights that all round to nothing)
+            if (part < 0) return false;
             above = sh.sum[0];
-#pragma unroll
-            for (int k = 0; k < PER; ++k)
-                if (key[k] >= klo && key[k] <= khi && (int)((khi - key[k]) >> shift) == part) atomicMin(&sh.key_lo, key[k]), atomicMax(&sh.key_hi, key[k]);
-            __syncthreads();
-            klo = sh.key_lo, khi = sh.key_hi;
+            khi -= (uint32_t)part << shift;
+            klo = max(klo, khi - min(khi, (1u << shift) - 1));
+            if (shift == 0) break;
             __syncthreads();
         }
-        K = klo;
+        K = KS ? klo << KS | (klo >> 15 ? 0u : 0xffffu) : klo;  // (negative values' keys are complements)
         // of K's equals, as many as start below what is wanted; one at least where nothing lies above
         const unsigned long long each = sample_weight(key_value(K), mx, r.c, p.shift);
         const double q = each ? ceil((want - (double)above) / (double)each) : 0.0;
@@ -666,8 +697,11 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
     // what each chunk keeps: its bins below the cut, the cut's keys above K, and its share of the ties
     __syncthreads();
     for (int c = w; c < p.C; c += ST / 64) {
-        unsigned long long t = 0;
-        for (int b = lane; b < lo; b += 64) t += hist[(long)c * NB + b];
+        unsigned long long t = 0, h[NB / 64];
+#pragma unroll
+        for (int k = 0; k < NB / 64; ++k) h[k] = lane + 64 * k < lo ? hist[(long)c * NB + lane + 64 * k] : 0;
+#pragma unroll
+        for (int k = 0; k < NB / 64; ++k) t += h[k];
         for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o, WAVE);
         if (lane == 0) sh.sums[c] = t, sh.tie[c] = 0;
     }
@@ -696,10 +730,11 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
     const double target = r.u * (double)total;
     if (mine && !((double)start > target) && (double)(start + mine) > target) sh.at[3] = tid, sh.sum[1] = start;
     __syncthreads();
-    // that chunk's logits in 16 stretches, a wave each: what they keep, then the one with the target
+    // That chunk's logits, a stretch of neighbours a thread: what each keeps, the thread that holds
+    // the target, and then its logits by the lanes of its wave.
     const int c0 = sh.at[3] * p.chunk, c1 = min(p.V, c0 + p.chunk);
-    const int per = ((c1 - c0 + ST / 64 - 1) / (ST / 64) + 63) / 64 * 64;
-    const int i0 = min(c1, c0 + w * per), i1 = min(c1, i0 + per);
+    constexpr int Q = 16;  // a stretch; chunks of up to 16384 logits
+    const int i0 = c0 + tid * Q;
     // a logit's weight if it is kept, or whether it is one of K's equals that count
     auto weigh = [&](float v, bool &tie) {
         const uint32_t key = sample_key(v);
@@ -708,65 +743,62 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
         tie = in && K && key == K;
         return in && !tie ? sample_weight(v, mx, r.c, p.shift) : 0ull;
     };
-    constexpr int U = 8;  // loads in flight
-    float v[U];
-    auto fetch = [&](int i) {
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const int at = i + 64 * k + lane;
-            v[k] = logit(min(at, p.V - 1));
-            if (at >= i1) v[k] = -INFINITY;
-        }
-    };
     unsigned long long m = 0;
     unsigned t = 0;
-    for (int i = i0; i < i1; i += 64 * U) {
-        fetch(i);
+    if (i0 < c1) {
+        float v[Q];
+        if (p.vec && i0 + Q <= c1) {
+            constexpr int E = 16 / sizeof(T);
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
+            for (int k = 0; k < Q / E; ++k) {
+                const u32x4 u = *(const u32x4 *)(x + i0 + k * E);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if constexpr (sizeof(T) == 4) v[k * E + e] = __uint_as_float(u[e]);
+                    else v[k * E + e] = __uint_as_float(e % 2 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
+                    v[k * E + e] = fmaxf(v[k * E + e], -INFINITY);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < Q; ++k) v[k] = i0 + k < c1 ? logit(i0 + k) : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
             bool tie;
             m += weigh(v[k], tie);
             t += tie;
         }
     }
-    for (int o = 32; o; o >>= 1) m += __shfl_xor(m, o, WAVE), t += __shfl_xor(t, o, WAVE);
-    if (lane == 0) sh.wave_sum[w] = m, sh.wave_ties[w] = t;
-    __syncthreads();
     const unsigned long long each = K ? sample_weight(key_value(K), mx, r.c, p.shift) : 0;
-    unsigned long long run = sh.sum[1];
     unsigned seen = sh.tie[sh.at[3]];  // K's equals before this stretch
-    for (int k = 0; k <= w; ++k) {
-        const unsigned long long kept = sh.wave_sum[k] + (seen < ties ? min(sh.wave_ties[k], ties - seen) : 0) * each;
-        if (k == w) m = kept;
-        else run += kept, seen += sh.wave_ties[k];
+    if (each) {
+        unsigned long long all;
+        seen += (unsigned)block_scan(t, sh.red, all);
+        m += (seen < ties ? min(t, ties - seen) : 0) * each;
     }
-    if (!m || (double)run > target || !((double)(run + m) > target)) return true;
-    for (int i = i0; i < i1; i += 64 * U) {  // one wave is left
-        fetch(i);
-#pragma unroll 1
-        for (int k = 0; k < U; ++k) {
-            float vk = v[0];
-#pragma unroll
-            for (int q = 1; q < U; ++q) vk = k == q ? v[q] : vk;
-            bool tie;
-            unsigned long long wt = weigh(vk, tie);
-            const unsigned long long eq = __builtin_amdgcn_ballot_w64(tie);
-            if (tie && seen + __popcll(eq & ((1ull << lane) - 1)) < ties) wt = each;
-            seen += __popcll(eq);
-            unsigned long long inc = wt;
-            for (int o = 1; o < 64; o <<= 1) {
-                const unsigned long long below = __shfl_up(inc, o, WAVE);
-                if (lane >= o) inc += below;
-            }
-            const unsigned long long hit = __builtin_amdgcn_ballot_w64(wt && (double)(run + inc) > target);
-            if (hit) {
-                if (lane == __ffsll((long long)hit) - 1) {
-                    p.ids[row] = i + 64 * k + lane;
-                    if (p.logp) p.logp[row] = (float)(sample_z(sc, vk) - log((double)total / sc.unit));
-                }
-                return true;
-            }
-            run += __shfl(inc, 63, WAVE);
+    unsigned long long all;
+    const unsigned long long run = sh.sum[1] + block_scan(m, sh.red, all);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(m && !((double)run > target) && (double)(run + m) > target);
+    if (!hit) return true;
+    {  // one wave is left: lane k has the stretch's logit k
+        const int from = __builtin_ctzll(hit), at = __builtin_amdgcn_readlane(i0, from) + lane;
+        const unsigned before = (unsigned)__builtin_amdgcn_readlane((int)seen, from);
+        const unsigned long long base = __shfl(run, from, WAVE);
+        const float v = lane < Q && at < c1 ? logit(at) : -INFINITY;
+        bool tie;
+        unsigned long long wt = weigh(v, tie);
+        const unsigned long long eq = __builtin_amdgcn_ballot_w64(tie);
+        if (tie && before + __popcll(eq & ((1ull << lane) - 1)) < ties) wt = each;
+        unsigned long long inc = wt;
+        for (int o = 1; o < Q; o <<= 1) {
+            const unsigned long long below = __shfl_up(inc, o, WAVE);
+            if (lane >= o) inc += below;
+        }
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(wt && (double)(base + inc) > target);
+        if (past && lane == __builtin_ctzll(past)) {
+            p.ids[row] = at;
+            if (p.logp) p.logp[row] = (float)(sample_z(sc, v) - log((double)total / sc.unit));
         }
     }
     return true;
@@ -786,11 +818,11 @@ __global__ void __launch_bounds__(ST) sample_finish_kernel(const SampleArgs p)
 
 using namespace jas;
 
-// Chunks of a row: of at least 4096 logits (a histogram of 12 KB each), until some 1024 workgroups
-// have one
+// Chunks of a row: of 4096 logits (a histogram of 12 KB each) up to 16384 (what the last step
+// walks at once), as many as give some 1024 workgroups one
 static void sample_chunks(int n, int V, int &C, int &chunk)
 {
-    C = std::max(1, std::min({(1024 + n - 1) / n, (V + 4095) / 4096, MAX_CHUNKS}));
+    C = std::max(std::min((1024 + n - 1) / n, (V + 4095) / 4096), (V + 16383) / 16384);
     chunk = ((V + C - 1) / C + 1023) / 1024 * 1024;
     C = (V + chunk - 1) / chunk;
 }
