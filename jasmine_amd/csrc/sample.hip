@@ -98,6 +98,19 @@ __device__ __forceinline__ float bin_edge(int b)
     return b <= 0 ? 0.f : b >= NB ? INFINITY : __uint_as_float((uint32_t)(b - 1 + (0x3c800000 >> 17)) << 17);
 }
 
+// Values that no logit of a bin lies above, or below: mx less the bin's edge, and 2^-20 of each more
+// than the subtractions' roundings
+__device__ __forceinline__ float bin_top(float mx, int b)
+{
+    const float t = mx - bin_edge(b) * (1 - 0x1p-20f);
+    return t + fabsf(t) * 0x1p-20f;
+}
+__device__ __forceinline__ float bin_bottom(float mx, int b)
+{
+    const float t = mx - bin_edge(b + 1) * (1 + 0x1p-20f);
+    return t - fabsf(t) * 0x1p-20f;
+}
+
 // Weight 2^shift e^((x - max) / T) as a whole number: c = log2(e) / T; 2^f by its series, |f| <= 1/2
 // (to 2^-47), and rounded by an addition of 2^52 (shift <= 51)
 __device__ __forceinline__ unsigned long long sample_weight(float x, double mx, double c, int shift)
@@ -125,23 +138,25 @@ struct SampleRow {
     int top_k;      // 0: all
     float top_p;    // 1: all
     double min_p, u;
-    bool greedy, plain;  // the first maximum; 1 / T and the maximum are finite
+    bool greedy, plain;  // the first maximum; 1 / T is finite
     double c;       // log2(e) / T
 };
-__device__ __forceinline__ SampleRow sample_row(const SampleArgs &p, int row, float mx)
+__device__ __forceinline__ SampleRow sample_row(const SampleArgs &p, int row)
 {
+    // (five loads in flight: an absent array's is one of u)
+    const float u = p.u[row], temp = *(p.temp ? p.temp + row : p.u), top_p = *(p.top_p ? p.top_p + row : p.u),
+                min_p = *(p.min_p ? p.min_p + row : p.u);
+    const int32_t top_k = *(p.top_k ? p.top_k + row : (const int32_t *)p.u);
     SampleRow r;
-    r.temp = p.temp ? p.temp[row] : 1.f;
-    r.top_k = p.top_k ? p.top_k[row] : 0;
+    r.temp = p.temp ? temp : 1.f;
+    r.top_k = p.top_k ? top_k : 0;
     if (r.top_k <= 0 || r.top_k >= p.V) r.top_k = 0;
     r.greedy = !(r.temp > 0.f) || r.top_k == 1;
-    r.top_p = p.top_p ? p.top_p[row] : 1.f;
-    if (!(r.top_p < 1.f)) r.top_p = 1.f;
-    r.min_p = p.min_p && p.min_p[row] > 0.f ? fmin((double)p.min_p[row], 1.0) : 0.0;
-    const float u = p.u[row];
+    r.top_p = p.top_p && top_p < 1.f ? top_p : 1.f;
+    r.min_p = p.min_p && min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
     r.u = !(u > 0.f) ? 0.f : fminf(u, 0x1.fffffep-1f);
     r.c = 1.4426950408889634074 / (double)r.temp;
-    r.plain = r.c > 0.0 && r.c < 1e300 && fabsf(mx) <= 3.402823466e38f;
+    r.plain = r.c > 0.0 && r.c < 1e300;
     return r;
 }
 
@@ -230,13 +245,12 @@ __global__ void __launch_bounds__(256) sample_hist_kernel(const SampleArgs p)
 {
     __shared__ unsigned long long bins[NB];
     const int row = blockIdx.y, c = blockIdx.x;
+    const SampleRow r = sample_row(p, row);
     uint32_t kmax;
     int imax;
     row_max_key(p, row, kmax, imax);
-    if (kmax == 0u) return;
     const float mx = key_value(kmax);
-    const SampleRow r = sample_row(p, row, mx);
-    if (r.greedy || !r.plain || r.top_k > SMALL_K) return;
+    if (kmax == 0u || mx == INFINITY || r.greedy || !r.plain || r.top_k > SMALL_K) return;
     for (int b = threadIdx.x; b < NB; b += 256) bins[b] = 0;
     __syncthreads();
     const T *x = (const T *)p.x + (long)row * p.ld;
@@ -501,6 +515,7 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
 {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const T *x = (const T *)p.x + (long)row * p.ld;
+    const SampleRow r = sample_row(p, row);
     uint32_t kmax;
     int imax;
     row_max_key(p, row, kmax, imax);
@@ -512,7 +527,6 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
         return true;
     }
     const float mx = key_value(kmax);
-    const SampleRow r = sample_row(p, row, mx);
     if (r.greedy) {
         if (tid == 0) {
             p.ids[row] = imax;
@@ -520,7 +534,7 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
         }
         return true;
     }
-    if (!r.plain || r.top_k > SMALL_K) return false;
+    if (mx == INFINITY || !r.plain || r.top_k > SMALL_K) return false;
     const SampleScale sc = {(double)mx, (double)r.temp, ldexp(1.0, p.shift), false};
     const unsigned long long *hist = p.hist + (long)row * p.C * NB;
     auto logit = [&](int i) {
@@ -536,8 +550,7 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
         __syncthreads();
         if (tid == 0) sh.n = 0;
         __syncthreads();
-        const float top = mx - bin_edge(lo) * (1 - 0x1p-20f), bottom = mx - bin_edge(hi + 1) * (1 + 0x1p-20f);
-        const float vtop = top + fabsf(top) * 0x1p-20f, vbottom = bottom - fabsf(bottom) * 0x1p-20f;
+        const float vtop = bin_top(mx, lo), vbottom = bin_bottom(mx, hi);
         auto look = [&](int at) {
             const float v = logit(at);
             const int b = sample_bin(mx - v);
@@ -575,21 +588,18 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
     };
     // the chunks' bins together, and the bin where their sum reaches what is wanted
     unsigned long long total = 0;
-    for (int b = tid; b < NB; b += ST) {
-        unsigned long long t = 0;
-        for (int c = 0; c < p.C; c += 8) {
-            unsigned long long h[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) h[k] = c + k < p.C ? hist[(long)(c + k) * NB + b] : 0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) t += h[k];
-        }
-        sh.sums[b] = t;
-    }
     if (tid == 0) sh.at[0] = -1;
-    __syncthreads();
     {
-        const unsigned long long a = 2 * tid < NB ? sh.sums[2 * tid] : 0, b = 2 * tid + 1 < NB ? sh.sums[2 * tid + 1] : 0;
+        typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+        unsigned long long a = 0, b = 0;  // bins 2 tid, 2 tid + 1
+        if (2 * tid < NB)
+            for (int c = 0; c < p.C; c += 8) {
+                u64x2 h[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) h[k] = c + k < p.C ? *(const u64x2 *)(hist + (long)(c + k) * NB + 2 * tid) : u64x2{0, 0};
+#pragma unroll
+                for (int k = 0; k < 8; ++k) a += h[k][0], b += h[k][1];
+            }
         const unsigned long long before = block_scan(a + b, sh.red, total);
         const double want = r.top_k ? (double)r.top_k : (double)r.top_p * (double)total;
         if (r.top_k || r.top_p < 1.f) {  // (one thread finds it)
@@ -649,8 +659,7 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
             wt[k] = i < n ? sample_weight(key_value(key[k]), mx, r.c, p.shift) : 0;
             key[k] >>= KS;
         }
-        const float top = mx - bin_edge(lo) * (1 - 0x1p-20f), bottom = lo == NB - 1 ? -3.402823466e38f : mx - bin_edge(lo + 1) * (1 + 0x1p-20f);
-        uint32_t khi = sample_key(top + fabsf(top) * 0x1p-20f) >> KS, klo = max(sample_key(bottom - fabsf(bottom) * 0x1p-20f) >> KS, 1u);
+        uint32_t khi = sample_key(bin_top(mx, lo)) >> KS, klo = max(sample_key(bin_bottom(mx, lo)) >> KS, 1u);
         while (true) {
             const int shift = klo == khi ? 0 : max(0, 22 - __builtin_clz(khi - klo));  // (khi - klo) >> shift < 1024
             sh.sums[tid] = 0;
@@ -735,12 +744,18 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
     const int c0 = sh.at[3] * p.chunk, c1 = min(p.V, c0 + p.chunk);
     constexpr int Q = 16;  // a stretch; chunks of up to 16384 logits
     const int i0 = c0 + tid * Q;
-    // a logit's weight if it is kept, or whether it is one of K's equals that count
+    // a logit's weight if it is kept, or whether it is one of K's equals that count; most are
+    // above or below the cut's bins for certain
+    const float sure = lo == NB ? -INFINITY : bin_top(mx, lo), never = lo == NB ? -INFINITY : bin_bottom(mx, hi);
     auto weigh = [&](float v, bool &tie) {
-        const uint32_t key = sample_key(v);
-        const int bin = sample_bin(mx - v);
-        const bool in = key && (bin < lo || (bin <= hi && key >= K && heavy(v, bin)));
-        tie = in && K && key == K;
+        bool in = v > sure;
+        tie = false;
+        if (v <= sure && v >= never && v > -INFINITY) {
+            const uint32_t key = sample_key(v);
+            const int bin = sample_bin(mx - v);
+            in = bin < lo || (bin <= hi && key >= K && heavy(v, bin));
+            tie = in && bin >= lo && K && key == K;
+        }
         return in && !tie ? sample_weight(v, mx, r.c, p.shift) : 0ull;
     };
     unsigned long long m = 0;
