@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
     constexpr int EV = D == 128 ? 4 : 2, NH = D / (16 * EV), KC = CD * NJ / 4;  // V: units of 32 keys x 16 EV d; K: KC steps a wave
     using KO = KOperand<KC * 32, CK>;
     using VO = VOperand<CK, EV>;
-    constexpr int ES = cache_bytes<CK>, LD = D + 4;
+    constexpr int ES = cache_bytes<CK>, LD = D + 4, RING = NK == 3 || CK >= CK_I8 ? 2 : 4;  // (as many as registers leave room for)
     constexpr bool EIGHT = CK >= CK_I8, ONES = NP == 1 && !EIGHT;  // row sums as P^T times ones
     static_assert(NJ == 4 || (NJ == 2 && CK == CK_F32), "a wave stages one block of 16 keys, or half of its d");
     __shared__ u32x4 Ks[NB][NK][NJ * CD * 64];
@@ -838,17 +838,32 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
         __syncthreads();
         gload(at ^ 1);
         if (kv0 >= wave_end) continue;  // nothing that a row of this wave sees
+        // Fragments of K, then of V, pass through a ring of registers, RING - 1 of them in flight: a
+        // read takes about 200 cycles with four waves at it, the products of one fragment 16 to
+        // 96.  (The fences keep the compiler from moving a read down to its use.)
+        bf16x8 ring[RING][NK];
+        auto fetch_k = [&](int f) {  // step f: 32 d, 16 keys
+#pragma unroll
+            for (int k = 0; k < NK; ++k) ring[f % RING][k] = as_bf16x8(Ks[buf][k][(f % NJ * CD + f / NJ) * 64 + lane]);
+        };
+        auto fetch_v = [&](int f) {  // step f: 32 keys, 16 d
+#pragma unroll
+            for (int k = 0; k < NK; ++k) ring[f % RING][k] = as_bf16x8(Vs[buf][k][(f % NC * NM + f / NC) * 64 + lane]);
+        };
         floatx4 s[NJ][NQ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int f = 0; f < RING - 1; ++f) fetch_k(f);
 #pragma unroll
-            for (int c = 0; c < CD; ++c) {
-                bf16x8 kf[NK];
+        for (int f = 0; f < NJ * CD; ++f) {
+            if (f + RING - 1 < NJ * CD) fetch_k(f + RING - 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int k = 0; k < NK; ++k) kf[k] = as_bf16x8(Ks[buf][k][(j * CD + c) * 64 + lane]);
+            for (int a = 0; a < NQ; ++a)
+                s[f % NJ][a] = mfma_planes(ring[f % RING], qf[a][f / NJ], f < NJ ? floatx4{0.f, 0.f, 0.f, 0.f} : s[f % NJ][a]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
-                for (int a = 0; a < NQ; ++a) s[j][a] = mfma_planes(kf, qf[a][c], c == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : s[j][a]);
-            }
+        for (int f = 0; f < RING - 1; ++f) fetch_v(f);
         floatx4 vsc[NJ];
         if (EIGHT) {
 #pragma unroll
@@ -911,16 +926,15 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
                 if (ONES) lacc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[m][a][0], lacc[a], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int f = 0; f < NC * NM; ++f) {
+            if (f + RING - 1 < NC * NM) fetch_v(f + RING - 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int m = 0; m < NM; ++m) {
-                bf16x8 vf[NK];
-#pragma unroll
-                for (int k = 0; k < NK; ++k) vf[k] = as_bf16x8(Vs[buf][k][(c * NM + m) * 64 + lane]);
-#pragma unroll
-                for (int a = 0; a < NQ; ++a) oacc[c][a] = mfma_planes(vf, pf[m][a], oacc[c][a]);
-            }
+            for (int a = 0; a < NQ; ++a) oacc[f % NC][a] = mfma_planes(ring[f % RING], pf[f / NC][a], oacc[f % NC][a]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
 #pragma unroll
