@@ -84,6 +84,46 @@ constexpr int SMALL_K = 1024; // largest top_k whose kept logits are sorted whol
 constexpr int CAP = 4096;     // logits that a row's cut may gather
 constexpr int MAX_CHUNKS = 1024;
 
+// Sums and extremes over a wave without LDS: rows of 16 lanes by DPP shifts, the rows by scalars
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t x, uint32_t none)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ unsigned long long dpp_u64(unsigned long long x)
+{
+    return (unsigned long long)dpp_u32<CTRL>((uint32_t)(x >> 32), 0u) << 32 | dpp_u32<CTRL>((uint32_t)x, 0u);
+}
+__device__ __forceinline__ unsigned long long lane_u64(unsigned long long x, int lane)
+{
+    return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+__device__ __forceinline__ unsigned long long row_scan(unsigned long long v)  // lanes up to one's own, of its 16
+{
+    v += dpp_u64<0x111>(v);  // row_shr
+    v += dpp_u64<0x112>(v);
+    v += dpp_u64<0x114>(v);
+    return v + dpp_u64<0x118>(v);
+}
+__device__ __forceinline__ unsigned long long wave_scan(unsigned long long v)
+{
+    v = row_scan(v);
+    const int row = (threadIdx.x & 63) >> 4;
+    const unsigned long long a = lane_u64(v, 15), b = a + lane_u64(v, 31), c = b + lane_u64(v, 47);
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
+{
+    v = max(v, dpp_u32<0x111>(v, 0u));
+    v = max(v, dpp_u32<0x112>(v, 0u));
+    v = max(v, dpp_u32<0x114>(v, 0u));
+    v = max(v, dpp_u32<0x118>(v, 0u));
+    const auto at = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); };
+    return max(max(at(15), at(31)), max(at(47), at(63)));
+}
+
 // Bin of d = max - x >= 0: below 2^-6 the first, then 64 to a doubling, the last from 2^17.9 up.
 // It does not fall as x falls.
 __device__ __forceinline__ int sample_bin(float d)
@@ -237,7 +277,9 @@ __device__ __forceinline__ void row_max_key(const SampleArgs &p, int row, uint32
 {
     k = 0, i = 0x7fffffff;
     for (int c = threadIdx.x & 63; c < p.C; c += 64) key_combine(k, i, p.chunk_key[(long)row * p.C + c], p.chunk_idx[(long)row * p.C + c]);
-    for (int o = 32; o; o >>= 1) key_combine(k, i, (uint32_t)__shfl_xor((int)k, o, WAVE), __shfl_xor(i, o, WAVE));
+    const uint32_t own = k;
+    k = wave_max_u32(k);
+    i = (int)~wave_max_u32(own == k ? ~(uint32_t)i : 0u);  // the least index among the largest
 }
 
 template <typename T>
@@ -265,25 +307,18 @@ __global__ void __launch_bounds__(256) sample_hist_kernel(const SampleArgs p)
     for (int b = threadIdx.x; b < NB; b += 256) out[b] = bins[b];
 }
 
-// first of the ST threads' 64-bit sums in thread order: exclusive prefix and total
+// The ST threads' 64-bit sums in thread order: exclusive prefix and total
 __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long *red, unsigned long long &total)
 {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    unsigned long long inc = v;
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long t = __shfl_up(inc, o, WAVE);
-        if (lane >= o) inc += t;
-    }
+    static_assert(ST == 1024, "a wave's sum in each of 16 lanes");
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned long long inc = wave_scan(v);
     __syncthreads();
     if (lane == 63) red[w] = inc;
     __syncthreads();
-    unsigned long long before = 0, all = 0;
-    for (int i = 0; i < ST / 64; ++i) {
-        if (i < w) before += red[i];
-        all += red[i];
-    }
-    total = all;
-    return before + inc - v;
+    const unsigned long long sums = row_scan(red[lane & 15]);
+    total = lane_u64(sums, 15);
+    return (w ? lane_u64(sums, w - 1) : 0) + inc - v;
 }
 
 // A row by one workgroup, whatever it holds: K by four passes of eight bits over the keys, each for
@@ -470,14 +505,19 @@ __device__ __attribute__((noinline)) void sample_row_general(const SampleArgs &p
 // larger ones of each, more by bitonic exchanges (s has room for the next power of two)
 __device__ __forceinline__ void sort_falling(unsigned long long *s, int n)
 {
-    if (n <= 256) {
-        const int i = threadIdx.x;
+    if (n <= 256) {  // a wave counts for 64 entries, over a quarter of the list
+        const int i = threadIdx.x & 255, part = threadIdx.x >> 8;
         const unsigned long long e = i < n ? s[i] : 0;
         int rank = 0;
-        if (i < (n + 63) / 64 * 64)
-            for (int j = 0; j < n; ++j) rank += s[j] > e;
+        if ((i & ~63) < n)
+#pragma unroll 8
+            for (int j = part; j < n; j += 4) rank += s[j] > e;
+        __shared__ int ranks[256];
+        if (part == 0) ranks[i] = rank;
         __syncthreads();
-        if (i < n) s[rank] = e;
+        if (part && rank) atomicAdd(&ranks[i], rank);
+        __syncthreads();
+        if (part == 0 && i < n) s[ranks[i]] = e;
         __syncthreads();
         return;
     }
@@ -711,8 +751,8 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
         for (int k = 0; k < NB / 64; ++k) h[k] = lane + 64 * k < lo ? hist[(long)c * NB + lane + 64 * k] : 0;
 #pragma unroll
         for (int k = 0; k < NB / 64; ++k) t += h[k];
-        for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o, WAVE);
-        if (lane == 0) sh.sums[c] = t, sh.tie[c] = 0;
+        t = wave_scan(t);
+        if (lane == 63) sh.sums[c] = t, sh.tie[c] = 0;
     }
     __syncthreads();
     for (int i = tid; i < n; i += ST) {
@@ -799,17 +839,13 @@ __device__ __forceinline__ bool sample_finish(const SampleArgs &p, int row, Fini
     {  // one wave is left: lane k has the stretch's logit k
         const int from = __builtin_ctzll(hit), at = __builtin_amdgcn_readlane(i0, from) + lane;
         const unsigned before = (unsigned)__builtin_amdgcn_readlane((int)seen, from);
-        const unsigned long long base = __shfl(run, from, WAVE);
+        const unsigned long long base = lane_u64(run, from);
         const float v = lane < Q && at < c1 ? logit(at) : -INFINITY;
         bool tie;
         unsigned long long wt = weigh(v, tie);
         const unsigned long long eq = __builtin_amdgcn_ballot_w64(tie);
         if (tie && before + __popcll(eq & ((1ull << lane) - 1)) < ties) wt = each;
-        unsigned long long inc = wt;
-        for (int o = 1; o < Q; o <<= 1) {
-            const unsigned long long below = __shfl_up(inc, o, WAVE);
-            if (lane >= o) inc += below;
-        }
+        const unsigned long long inc = row_scan(wt);
         const unsigned long long past = __builtin_amdgcn_ballot_w64(wt && (double)(base + inc) > target);
         if (past && lane == __builtin_ctzll(past)) {
             p.ids[row] = at;
