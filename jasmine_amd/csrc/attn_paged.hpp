@@ -37,7 +37,7 @@ struct PagedAttnArgs {
     float scale_log2;
     int q_vec, o_vec;           // rows of Q, O start on 16 bytes
     int tiles, nsplit, chunk;   // grid: tiles x nsplit x key heads; keys of a split, at least
-    int sorted, cus;            // tiles in order of falling length; compute units
+    int sorted, cus;            // tiles in order of falling length; compute units, if two tiles share one
     float *part;                // nsplit > 1: rows of D means, then exponent base and sum
 };
 
@@ -79,16 +79,14 @@ struct PagedSeq {
 // Tile x of the grid: sequence b owns tiles from floor(cu[b] G / M) + b on, at least as many as
 // its rows fill, so the thread that holds b knows it from cu[b] and cu[b + 1] alone: one round of
 // loads, no running sum.  Returns x's tile number in b, or -1.  By the whole workgroup.
-template <int M>
+template <int M, int NT>
 __device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
 {
     __shared__ int s_b, s_seq[4];
     if (threadIdx.x == 0) s_b = -1, s_seq[3] = -1;
     __syncthreads();
     int own = -2, row0 = 0, rows = 0, len = 0, at = 0;
-    for (int j0 = 0; j0 < p.bt.B; j0 += 256) {
-        const int j = j0 + (int)threadIdx.x;
-        if (j >= p.bt.B) break;
+    for (int j = threadIdx.x; j < p.bt.B; j += NT) {
         const int c0 = max(0, min(p.bt.cu[j], p.bt.n)), c1 = max(c0, min(p.bt.cu[j + 1], p.bt.n)), n = p.bt.lens[j];
         const int first = (int)((long)c0 * p.G / M + j);
         if (first <= x && (j + 1 == p.bt.B || (int)((long)c1 * p.G / M + j + 1) > x))
@@ -105,12 +103,13 @@ __device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b,
 
 // The same in order of falling length, for launches whose workgroups own whole sequences of keys (B
 // <= 256): each thread adds the tiles of the sequences before its own.  Workgroups start in the order
-// of their ids, i and i + C (C compute units) on one unit where two fit, so the second C of them
-// are taken from the light end: 8 chunks of up to 256 beside 16 decoding sequences, 148 -> 122 us.
+// of their ids; where two fit on a unit, i and i + cus share one, so the second cus of them are
+// taken from the light end (cus 0: they do not): 8 chunks of up to 256 beside 16 decoding sequences,
+// 148 -> 122 us.
 template <int M>
 __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
 {
-    __shared__ int s_tiles[256], s_len[256], s_seq[4];
+    __shared__ int s_tiles[256], s_len[256], s_seq[5];
     const int j = threadIdx.x;
     int row0 = 0, rows = 0, len = 0;
     if (j < p.bt.B) {
@@ -119,8 +118,8 @@ __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, 
         len = max(0, min(p.bt.lens[j], min(p.kv.cap, p.max_len)));
     }
     const int tiles = (int)(((long)rows * p.G + M - 1) / M);
-    s_tiles[j] = tiles, s_len[j] = len;
-    if (j == 0) s_seq[3] = -1;
+    if (j < 256) s_tiles[j] = tiles, s_len[j] = len;
+    if (j == 0) s_seq[3] = -1, s_seq[4] = 0;
     __syncthreads();
     int first = 0, total = 0;
     for (int k = 0; k < p.bt.B; ++k) {
@@ -130,10 +129,9 @@ __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, 
     }
     const int lo = p.cus / p.kv.n_kv, hi = min(2 * lo, total);  // tiles of the first and second round
     if (x >= lo && x < hi) x = lo + hi - 1 - x;
-    if (x >= first && x < first + tiles) s_seq[0] = row0, s_seq[1] = rows, s_seq[2] = len, s_seq[3] = x - first, s_tiles[0] = j;
+    if (x >= first && x < first + tiles) s_seq[0] = row0, s_seq[1] = rows, s_seq[2] = len, s_seq[3] = x - first, s_seq[4] = j;
     __syncthreads();
-    sq.row0 = s_seq[0], sq.rows = s_seq[1], sq.len = s_seq[2];
-    b = max(0, min(s_tiles[0], p.bt.B - 1));
+    sq.row0 = s_seq[0], sq.rows = s_seq[1], sq.len = s_seq[2], b = s_seq[4];
     return s_seq[3];
 }
 
@@ -243,12 +241,12 @@ __device__ __forceinline__ PagedRow paged_row_of(const PagedAttnArgs &p, const P
 }
 
 // Computes the rows of a tile again whose bit in bad[] is set: results or partial results
-template <int D, int CK, typename T>
+template <int D, int CK, typename T, int NW>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &p, int b, int hk, const PagedSeq &sq, int r0, int rows,
                                                       const unsigned *bad, int k_lo, int k_hi, float *part)
 {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int r = w; r < rows; r += 4) {
+    for (int r = w; r < rows; r += NW) {
         if (!(bad[r / 32] >> (r % 32) & 1)) continue;
         const PagedRow row = paged_row_of(p, sq, hk, r0 + r);
         float m, l, out[(D + 63) / 64];
@@ -281,32 +279,33 @@ struct KOperand {
         if (CK == CK_BF16 || D == 32) return 32 * c + 8 * g + j;
         return 64 * (c / 2) + 16 * g + 8 * (c % 2) + j;
     }
-    // row: the first element of the key; NT: a stream that is read once
-    template <bool NT = false>
-    static __device__ __forceinline__ void load(const void *row, int g, uint32_t (&r)[CD][RW])
+    // steps c0 .. c0 + KC - 1 of a key (row: its first element); NT: a stream that is read once
+    template <int KC, bool NT = false>
+    static __device__ __forceinline__ void load(const void *row, int g, int c0, uint32_t (&r)[KC][RW])
     {
-        const char *p = (const char *)row + (CK == CK_F32 || CK == CK_BF16 || D >= 64 ? 16 : 8) * g;
+        const char *p = (const char *)row;
         if constexpr (CK == CK_F32) {
 #pragma unroll
-            for (int c = 0; c < CD; ++c) {
-                const u32x4 a = cache_load<NT, u32x4>((p + 128 * c)), b = cache_load<NT, u32x4>((p + 128 * c + 64));
+            for (int c = 0; c < KC; ++c) {
+                const u32x4 a = cache_load<NT, u32x4>(p + 128 * (c0 + c) + 16 * g), b = cache_load<NT, u32x4>(p + 128 * (c0 + c) + 16 * g + 64);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) r[c][e] = a[e], r[c][4 + e] = b[e];
             }
         } else if constexpr (CK == CK_BF16) {
 #pragma unroll
-            for (int c = 0; c < CD; ++c) {
-                const u32x4 a = cache_load<NT, u32x4>((p + 64 * c));
+            for (int c = 0; c < KC; ++c) {
+                const u32x4 a = cache_load<NT, u32x4>(p + 64 * (c0 + c) + 16 * g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) r[c][e] = a[e];
             }
         } else if constexpr (D == 32) {
-            const u32x2 a = cache_load<NT, u32x2>(p);
+            const u32x2 a = cache_load<NT, u32x2>(p + 8 * g);
             r[0][0] = a[0], r[0][1] = a[1];
         } else {
+            static_assert(KC % 2 == 0, "pairs of steps lie together");
 #pragma unroll
-            for (int c = 0; c < CD; c += 2) {
-                const u32x4 a = cache_load<NT, u32x4>((p + 32 * c));
+            for (int c = 0; c < KC; c += 2) {
+                const u32x4 a = cache_load<NT, u32x4>(p + 32 * (c0 + c) + 16 * g);
                 r[c][0] = a[0], r[c][1] = a[1], r[c + 1][0] = a[2], r[c + 1][1] = a[3];
             }
         }
@@ -318,12 +317,11 @@ template <int CK>
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t w, bool hi)
 {
     if constexpr (CK == CK_F8) {
-        const auto v = hi ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-        // (bf16 numbers in fp32: their upper halves)
-        return __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
+        return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
     } else {
         const int sh = hi ? 16 : 0;
         const float a = (float)(int8_t)(w >> sh), b = (float)(int8_t)(w >> (sh + 8));
+        // (bf16 numbers in fp32: their upper halves)
         return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
     }
 }
@@ -487,7 +485,7 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
     const int hk = blockIdx.x % p.kv.n_kv, rest = blockIdx.x / p.kv.n_kv, split = rest % p.nsplit, x = rest / p.nsplit;
     int b;
     PagedSeq sq;
-    const int tile = paged_tile<M>(p, x, b, sq);
+    const int tile = paged_tile<M, 256>(p, x, b, sq);
     const int r0 = tile * M, rows = min(M, sq.rows * p.G - r0);
     if (tile < 0 || rows <= 0) return;
     const PagedRow row = paged_row_of(p, sq, hk, r0 + min(r16, rows - 1));
@@ -534,7 +532,7 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
     uint32_t kr[2][CD][KO::RW], vr[8][VO::RW];
     auto kload = [&]() {
 #pragma unroll
-        for (int a = 0; a < 2; ++a) KO::template load<true>(kpool + s_off[w][16 * a + r16], g, kr[a]);
+        for (int a = 0; a < 2; ++a) KO::template load<CD, true>(kpool + s_off[w][16 * a + r16], g, 0, kr[a]);
     };
     auto vload = [&]() {
 #pragma unroll
@@ -679,27 +677,31 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
         }
     }
     if (part && w == 0 && g == 0 && r16 < rows && !(bad >> r16 & 1)) part[(long)r16 * LD + D] = mm, part[(long)r16 * LD + D + 1] = ll;
-    if (bad) paged_again<D, CK, T>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
+    if (bad) paged_again<D, CK, T, 4>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
 }
 
 // ---------------------------------------------------------------- many rows: chunks
-// One workgroup: a tile of 64 NQ rows, 16 NQ a wave, and one split of its keys.  Tiles of BK keys go
+// One workgroup: a tile of 16 NQ NW rows, 16 NQ a wave of NW, and one split of its keys.  Tiles of BK keys go
 // through LDS in operand order (one ds_read_b128 a fragment, no bank conflict on either side): read
 // from their pages a tile ahead, widened or split once, V transposed by the lanes that stage it.
 // Where operands are single bf16 planes two buffers of LDS need one barrier a tile; three planes
 // take one buffer and two barriers.
-template <int D, int CK, typename T, int NQ>
-__global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs p)
+// 32 rows a wave read a fragment from LDS for twice the products; 16 leave registers for more waves,
+// which share out the widening of codes: bf16 rows over 8-bit caches at D = 128 (4 chunks of 512 over
+// 4096 keys, int8: 234 us with 32, 175 with 16; over bf16 139 and 147).
+template <int D, int CK, typename T, int NQ, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnArgs p)
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, NK = CK == CK_F32 ? 3 : 1, NB = NK == 3 ? 1 : 2;
-    constexpr int BK = NK == 3 && D == 128 ? 32 : 64, M = 64 * NQ;
+    constexpr int BK = NK == 3 && D == 128 ? 32 : 64, M = 16 * NQ * NW;
     constexpr int CD = D / 32, NC = D / 16, NJ = BK / 16, NM = BK / 32;
-    constexpr int EV = D == 128 ? 4 : 2, NH = D / (16 * EV), KC = CD * NJ / 4;  // V: units of 32 keys x 16 EV d; K: KC steps a wave
-    using KO = KOperand<KC * 32, CK>;
+    constexpr int EV = D == 128 && NW == 4 ? 4 : 2, NH = D / (16 * EV), NU = NM * NH;  // V: units of 32 keys x 16 EV d
+    constexpr int KC = CD * NJ / NW;  // K: a wave stages KC steps of 16 keys
+    using KO = KOperand<D, CK>;
     using VO = VOperand<CK, EV>;
-    constexpr int ES = cache_bytes<CK>, LD = D + 4, RING = NK == 3 || CK >= CK_I8 ? 2 : 4;  // (as many as registers leave room for)
+    constexpr int ES = cache_bytes<CK>, LD = D + 4, RING = NK == 3 || (CK >= CK_I8 && NQ == 2) ? 2 : 4;  // (as many as registers leave room for)
     constexpr bool EIGHT = CK >= CK_I8, ONES = NP == 1 && !EIGHT;  // row sums as P^T times ones
-    static_assert(NJ == 4 || (NJ == 2 && CK == CK_F32), "a wave stages one block of 16 keys, or half of its d");
+    static_assert(NW % NJ == 0 && KC > 0, "a block of 16 keys is staged by NW / NJ waves");
     __shared__ u32x4 Ks[NB][NK][NJ * CD * 64];
     __shared__ u32x4 Vs[NB][NK][NC * NM * 64];
     __shared__ long s_off[2][64];
@@ -711,7 +713,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
     const int hk = blockIdx.x % p.kv.n_kv, rest = blockIdx.x / p.kv.n_kv, split = rest % p.nsplit, x = rest / p.nsplit;
     int b;
     PagedSeq sq;
-    const int tile = p.sorted ? paged_tile_sorted<M>(p, x, b, sq) : paged_tile<M>(p, x, b, sq);
+    const int tile = p.sorted ? paged_tile_sorted<M>(p, x, b, sq) : paged_tile<M, 64 * NW>(p, x, b, sq);
     const int r0 = tile * M, rows = min(M, sq.rows * p.G - r0);
     if (tile < 0 || rows <= 0) return;
     const int kend = paged_row_of(p, sq, hk, r0 + rows - 1).end;  // (the last row of a tile sees most)
@@ -738,9 +740,9 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
         q_planes<D, CK, T, NP>((const T *)p.q + row.tok * p.q_st + row.h * p.q_sh, r < rows, g, p.q_vec, qf[a]);
     }
 
-    const char *kpool = (const char *)p.kv.k + hk * p.kv.head_stride * ES + (NJ == 2 ? (w >> 1) * KC * 32 * ES : 0);
+    const char *kpool = (const char *)p.kv.k + hk * p.kv.head_stride * ES;
     const char *vpool = (const char *)p.kv.v + hk * p.kv.head_stride * ES + r16 * EV * ES;
-    const int kj = NJ == 2 ? w & 1 : w;  // this wave's block of keys
+    const int kj = w % NJ, kc = w / NJ * KC;  // this wave's block of keys, and its first step
     // the tile two ahead: its entries of the table (wave 0, one key a lane); one ahead: its places
     int page = 0, slot = 0;
     bool in = false;
@@ -764,13 +766,13 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
             }
         }
     };
-    uint32_t kr[KC][KO::RW], vr[(NM * NH + 3) / 4][8][VO::RW];
+    uint32_t kr[KC][KO::RW], vr[(NU + NW - 1) / NW][8][VO::RW];
     auto gload = [&](int at) {
-        KO::load(kpool + s_off[at][16 * kj + r16], g, kr);
+        KO::template load<KC>(kpool + s_off[at][16 * kj + r16], g, kc, kr);
 #pragma unroll
-        for (int q = 0; q < (NM * NH + 3) / 4; ++q) {
-            const int u = w + 4 * q;
-            if (NM * NH % 4 != 0 && u >= NM * NH) continue;
+        for (int q = 0; q < (NU + NW - 1) / NW; ++q) {
+            const int u = w + NW * q;
+            if (NU % NW != 0 && u >= NU) continue;
             const int mm = u / NH, h = u % NH;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -783,14 +785,14 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
         for (int c = 0; c < KC; ++c) {
             u32x4 pl[NK];
             k_planes<CK>(kr[c], pl);
-            const int u = kj * CD + (NJ == 2 ? (w >> 1) * KC : 0) + c;
+            const int u = kj * CD + kc + c;
 #pragma unroll
             for (int k = 0; k < NK; ++k) Ks[buf][k][u * 64 + lane] = pl[k];
         }
 #pragma unroll
-        for (int q = 0; q < (NM * NH + 3) / 4; ++q) {
-            const int u = w + 4 * q;
-            if (NM * NH % 4 != 0 && u >= NM * NH) continue;
+        for (int q = 0; q < (NU + NW - 1) / NW; ++q) {
+            const int u = w + NW * q;
+            if (NU % NW != 0 && u >= NU) continue;
             const int mm = u / NH, h = u % NH;
             if (valid != (BK == 64 ? ~0ull : 0xffffffffull)) {  // values of keys without a page, or past the end, are none
 #pragma unroll
@@ -984,7 +986,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
         if (part && g == 0) part[(long)r * LD + D] = ll != 0.f ? mb[a] : -INFINITY, part[(long)r * LD + D + 1] = ll;
     }
     __syncthreads();
-    if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) paged_again<D, CK, T>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
+    if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) paged_again<D, CK, T, NW>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
 }
 
 // Joins the splits of a tile's rows, one wave a row: lane i weighs split i (nsplit <= 64), then the
@@ -997,7 +999,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs p,
     const int quarter = blockIdx.x % (M / 4), rest = blockIdx.x / (M / 4), hk = rest % p.kv.n_kv, x = rest / p.kv.n_kv;
     int b;
     PagedSeq sq;
-    const int tile = M == 16 ? paged_tile<16>(p, x, b, sq) : M == 64 ? paged_tile<64>(p, x, b, sq) : paged_tile<128>(p, x, b, sq);
+    const int tile = M == 16 ? paged_tile<16, 256>(p, x, b, sq) : M == 64 ? paged_tile<64, 256>(p, x, b, sq) : paged_tile<128, 256>(p, x, b, sq);
     const int r = quarter * 4 + w;
     if (tile < 0 || r >= sq.rows * p.G - tile * M) return;
     const float *part = p.part + (((long)x * p.kv.n_kv + hk) * p.nsplit * M + r) * LD;
@@ -1039,8 +1041,12 @@ void paged_launch_as(const PagedAttnArgs &p, int rows, hipStream_t s)
 {
     const dim3 grid((unsigned)p.tiles * p.nsplit * p.kv.n_kv), block(256);
     if (rows == 16) hipLaunchKernelGGL((paged_stream_kernel<D, CK, T>), grid, block, 0, s, p);
-    else if (rows == 64) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1>), grid, block, 0, s, p);
-    else if constexpr (sizeof(T) == 2 || D < 128) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 2>), grid, block, 0, s, p);
+    else if (rows == 64) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1, 4>), grid, block, 0, s, p);
+    else if constexpr (D == 128 && CK >= CK_I8 && sizeof(T) == 2) {
+        PagedAttnArgs one = p;
+        one.cus = 0;  // (one workgroup a unit)
+        hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1, 8>), grid, dim3(512), 0, s, one);
+    } else if constexpr (sizeof(T) == 2 || D < 128) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 2, 4>), grid, block, 0, s, p);
     if (p.nsplit > 1) hipLaunchKernelGGL((paged_merge_kernel<D, T>), dim3((unsigned)p.tiles * p.kv.n_kv * (rows / 4)), block, 0, s, p, rows);
 }
 
