@@ -294,7 +294,7 @@ typedef struct {
 /* A ragged batch: of n rows of tokens, rows d_cu[b] .. d_cu[b + 1] - 1 are the last tokens of
  * sequence b, which has d_lens[b] tokens with them (d_cu: B + 1 non-decreasing device int32 from
  * 0; d_lens: B).  Row i of sequence b so stands at position d_lens[b] - d_cu[b + 1] + i.  Rows
- * from d_cu[B] on are not read and not written.  Positions below 0 or past the table's row are
+ * from d_cu[B] on have no effect and are not written.  Positions below 0 or past the table's row are
  * no tokens: not written, read as zeros.
  *
  * Writes the new tokens' keys and values (device, JAS_F32 or JAS_BF16, token stride st, head

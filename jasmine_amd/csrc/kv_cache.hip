@@ -69,7 +69,7 @@ __device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8])
 {
     if constexpr (sizeof(T) == 4) {
         if (vec) {
-            const floatx4 a = *(const floatx4 *)p, b = *(const floatx4 *)(p + 4);
+            const floatx4 a = __builtin_nontemporal_load((const floatx4 *)p), b = __builtin_nontemporal_load((const floatx4 *)(p + 4));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
         } else {
@@ -78,7 +78,7 @@ __device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8])
         }
     } else {
         if (vec) {
-            const u32x4 t = *(const u32x4 *)p;
+            const u32x4 t = __builtin_nontemporal_load((const u32x4 *)p);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(t[e] << 16), v[2 * e + 1] = __uint_as_float(t[e] & 0xffff0000u);
         } else {
@@ -150,24 +150,104 @@ __device__ __forceinline__ bool find_token(const BatchView &bt, const int32_t *c
 
 constexpr int CU_LDS = 1024;  // batches up to this size are searched in LDS
 
-// One thread: eight values of a row, of the keys (blockIdx.y = 0) or the values.  READ: cache to
-// rows, else rows to cache.
+// Eight values of the cache at element `at`, in fp32, and back
+template <int CK>
+__device__ __forceinline__ void cache_get(const void *pool, const float *scale, long at, long sc, float (&v)[8])
+{
+    if constexpr (CK == CK_F32) load8((const float *)pool + at, true, v);
+    else if constexpr (CK == CK_BF16) load8((const uint16_t *)pool + at, true, v);
+    else {
+        const float s = scale[sc];
+        const u32x2 c = *(const u32x2 *)((const uint8_t *)pool + at);
+        if constexpr (CK == CK_I8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(c[e / 4] >> (8 * (e & 3))) * s;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(c[e], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(c[e], true);
+                v[4 * e] = a[0] * s, v[4 * e + 1] = a[1] * s, v[4 * e + 2] = d[0] * s, v[4 * e + 3] = d[1] * s;
+            }
+        }
+    }
+}
+// (every lane of a row comes here, whether the row is stored or not: they meet in its maximum)
+template <int D, int CK>
+__device__ __forceinline__ void cache_put(void *pool, float *scale, long at, long sc, bool there, int l, const float (&v)[8])
+{
+    if constexpr (CK == CK_F32) {
+        if (there) store8((float *)pool + at, true, v);
+    } else if constexpr (CK == CK_BF16) {
+        if (there) store8((uint16_t *)pool + at, true, v);
+    } else {
+        // the row's largest magnitude; an infinity or NaN anywhere makes it one (fmaxf would drop a NaN)
+        float mx = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            mx = fmaxf(mx, fabsf(v[e]));
+            bad |= !(fabsf(v[e]) <= 3.402823466e38f);
+        }
+        mx = row_max<D / 8>(bad ? INFINITY : mx);
+        constexpr float QMAX = CK == CK_I8 ? 127.f : 448.f;
+        float s = mx / QMAX;
+        if (!(mx <= 3.402823466e38f)) s = __uint_as_float(0x7fc00000u);
+        else if (s < 0x1p-126f) s = 0.f;
+        // scaled into the middle of the range, where the residual of a quotient is exact
+        const float up = s < 0x1p-40f ? 0x1p80f : s > 0x1p40f ? 0x1p-80f : 1.f;
+        const float ss = s * up, inv = 1.0f / ss;
+        u32x2 c = {0, 0};
+        if (s > 0.f) {  // (a NaN scale too has codes of zero)
+            float q[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = quotient_to_odd(v[e] * up, ss, inv);
+            if constexpr (CK == CK_I8) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int k = (int)fminf(fmaxf(rintf(q[e]), -127.f), 127.f);
+                    c[e / 4] |= ((uint32_t)k & 255u) << (8 * (e & 3));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(q[e], -448.f), 448.f);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int t = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * e], q[4 * e + 1], 0, false);
+                    c[e] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4 * e + 2], q[4 * e + 3], t, true);
+                }
+            }
+        }
+        if (there) {
+            *(u32x2 *)((uint8_t *)pool + at) = c;
+            if (l == 0) scale[sc] = s;
+        }
+    }
+}
+
+// One thread: eight values of a row.  READ: cache to rows, of the keys and of the values, which lie
+// alike, so that one look into the table serves both.  Else rows to cache, of one of them (blockIdx.y:
+// the quantising is as long as the loads), read before the table is.
 template <int D, int CK, typename T, bool READ>
 __global__ void __launch_bounds__(256) kv_move_kernel(const KvArgs p)
 {
     constexpr int L = D / 8;
     __shared__ int32_t cu_s[CU_LDS + 1];
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    const int l = (int)(id % L);
+    const long row = id / L;
+    const int h = (int)(row % p.kv.n_kv);
+    const long tok = row / p.kv.n_kv;
+    const long from = tok * p.st + h * p.sh + 8 * l;
+    const int which = READ ? 0 : blockIdx.y;
+    float k[8], v[8];
+    // (whether the row is one of the batch is not known yet, but rows up to n are there to be read)
+    if (!READ && tok < p.bt.n) load8((const T *)p.x[which] + from, p.vec, k);
     const int32_t *cu = p.bt.cu;
     if (p.bt.B <= CU_LDS) {
         for (int i = threadIdx.x; i <= p.bt.B; i += 256) cu_s[i] = cu[i];
         __syncthreads();
         cu = cu_s;
     }
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    const int l = (int)(id % L);
-    const long row = id / L;
-    const int h = (int)(row % p.kv.n_kv);
-    const long tok = row / p.kv.n_kv;
     if (tok >= p.bt.n) return;
     int b, pos;
     if (!find_token(p.bt, cu, (int)tok, b, pos)) return;
@@ -178,96 +258,24 @@ __global__ void __launch_bounds__(256) kv_move_kernel(const KvArgs p)
         page = p.kv.table[(long)b * p.kv.table_stride + q];
     }
     const bool there = page >= 0 && page < p.kv.n_pages;
-    const int which = blockIdx.y;
-    T *x = (T *)p.x[which];
-    if (!x) return;
-    x += tok * p.st + h * p.sh + 8 * l;
     const long at = (long)page * p.kv.page_stride + h * p.kv.head_stride + slot * p.kv.tok_stride + 8 * l;
     const long sc = ((long)page * p.kv.n_kv + h) * p.kv.page_size + slot;
-    void *pool = which ? p.kv.v : p.kv.k;
-    float *scale = which ? p.kv.vs : p.kv.ks;
-    float v[8];
     if constexpr (READ) {
-        if (!there) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        } else if constexpr (CK == CK_F32) {
-            load8((const float *)pool + at, true, v);
-        } else if constexpr (CK == CK_BF16) {
-            load8((const uint16_t *)pool + at, true, v);
-        } else {
-            const float s = scale[sc];
-            const u32x2 c = *(const u32x2 *)((const uint8_t *)pool + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (CK == CK_I8) v[e] = (float)(int8_t)(c[e / 4] >> (8 * (e & 3))) * s;
-            }
-            if constexpr (CK == CK_F8) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(c[e], false), d = __builtin_amdgcn_cvt_pk_f32_fp8(c[e], true);
-                    v[4 * e] = a[0] * s, v[4 * e + 1] = a[1] * s, v[4 * e + 2] = d[0] * s, v[4 * e + 3] = d[1] * s;
-                }
-            }
-        }
-        store8(x, p.vec, v);
+        for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
+        if (there && p.x[0]) cache_get<CK>(p.kv.k, p.kv.ks, at, sc, k);
+        if (there && p.x[1]) cache_get<CK>(p.kv.v, p.kv.vs, at, sc, v);
+        if (p.x[0]) store8((T *)p.x[0] + from, p.vec, k);
+        if (p.x[1]) store8((T *)p.x[1] + from, p.vec, v);
     } else {
-        load8((const T *)x, p.vec, v);
-        if constexpr (CK == CK_F32) {
-            if (there) store8((float *)pool + at, true, v);
-        } else if constexpr (CK == CK_BF16) {
-            if (there) store8((uint16_t *)pool + at, true, v);
-        } else {
-            // the row's largest magnitude; an infinity or NaN anywhere makes it one (as whole
-            // numbers, magnitudes of NaN lie above infinity, and fmaxf would drop a NaN)
-            float mx = 0.f;
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                mx = fmaxf(mx, fabsf(v[e]));
-                bad |= !(fabsf(v[e]) <= 3.402823466e38f);
-            }
-            mx = row_max<L>(bad ? INFINITY : mx);
-            constexpr float QMAX = CK == CK_I8 ? 127.f : 448.f;
-            float s = mx / QMAX;
-            if (!(mx <= 3.402823466e38f)) s = __uint_as_float(0x7fc00000u);
-            else if (s < 0x1p-126f) s = 0.f;
-            // scaled into the middle of the range, where the residual of a quotient is exact
-            const float up = s < 0x1p-40f ? 0x1p80f : s > 0x1p40f ? 0x1p-80f : 1.f;
-            const float ss = s * up, inv = 1.0f / ss;
-            u32x2 c = {0, 0};
-            if (s > 0.f) {  // (a NaN scale too has codes of zero)
-                float q[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) q[e] = quotient_to_odd(v[e] * up, ss, inv);
-                if constexpr (CK == CK_I8) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int k = (int)fminf(fmaxf(rintf(q[e]), -127.f), 127.f);
-                        c[e / 4] |= ((uint32_t)k & 255u) << (8 * (e & 3));
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(q[e], -448.f), 448.f);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        int t = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * e], q[4 * e + 1], 0, false);
-                        c[e] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4 * e + 2], q[4 * e + 3], t, true);
-                    }
-                }
-            }
-            if (there) {
-                *(u32x2 *)((uint8_t *)pool + at) = c;
-                if (l == 0) scale[sc] = s;
-            }
-        }
+        cache_put<D, CK>(which ? p.kv.v : p.kv.k, which ? p.kv.vs : p.kv.ks, at, sc, there, l, k);
     }
 }
 
 template <int D, int CK, bool READ>
 static void kv_launch(const KvArgs &p, int dtype, hipStream_t s)
 {
-    const dim3 grid(ceil_div((long)p.bt.n * p.kv.n_kv * (D / 8), 256), 2), block(256);
+    const dim3 grid(ceil_div((long)p.bt.n * p.kv.n_kv * (D / 8), 256), READ ? 1 : 2), block(256);
     if (dtype == JAS_F32) hipLaunchKernelGGL((kv_move_kernel<D, CK, float, READ>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((kv_move_kernel<D, CK, uint16_t, READ>), grid, block, 0, s, p);
 }

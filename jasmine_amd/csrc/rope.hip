@@ -33,7 +33,7 @@ struct RopeIo<float> {
     static __device__ void put(float *p, float v) { *p = v; }
     static __device__ void get(const float *p, float (&v)[4])
     {
-        const floatx4 t = *(const floatx4 *)p;
+        const floatx4 t = __builtin_nontemporal_load((const floatx4 *)p);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = t[e];
     }
@@ -46,7 +46,7 @@ struct RopeIo<uint16_t> {
     static __device__ void put(uint16_t *p, float v) { *p = __builtin_bit_cast(uint16_t, (__bf16)v); }
     static __device__ void get(const uint16_t *p, float (&v)[8])
     {
-        const u32x4 t = *(const u32x4 *)p;
+        const u32x4 t = __builtin_nontemporal_load((const u32x4 *)p);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(t[e] << 16), v[2 * e + 1] = __uint_as_float(t[e] & 0xffff0000u);
     }
@@ -109,38 +109,35 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs p)
     const double pos = p.pos[tok];
 #pragma unroll
     for (int i = 0; i < NP; ++i) rope_angle(pos, p.freq[u * NP + i], p.mscale, c[i], s[i]);
+    if constexpr (VEC) {  // every head's loads, then its products
+        constexpr int P = HALVES ? 2 : 1;
+        float v[ROPE_HEADS][P][E];
 #pragma unroll
-    for (int k = 0; k < ROPE_HEADS; ++k) {
-        if (h0 + k >= h1) break;
-        const T *xr = x + (h0 + k) * p.x_sh;
-        T *yr = y + (h0 + k) * p.y_sh;
-        if constexpr (VEC && HALVES) {
-            float a[E], b[E];
-            Io::get(xr + u * E, a);
-            Io::get(xr + half + u * E, b);
+        for (int k = 0; k < ROPE_HEADS; ++k) {
+            const T *xr = x + min(h0 + k, h1 - 1) * p.x_sh + u * E;
+            Io::get(xr, v[k][0]);
+            if constexpr (HALVES) Io::get(xr + half, v[k][1]);
+        }
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float t = a[i] * c[i] - b[i] * s[i];
-                b[i] = a[i] * s[i] + b[i] * c[i];
-                a[i] = t;
-            }
-            Io::put(yr + u * E, a);
-            Io::put(yr + half + u * E, b);
-        } else if constexpr (VEC) {
-            float a[E];
-            Io::get(xr + u * E, a);
+        for (int k = 0; k < ROPE_HEADS; ++k) {
+            if (h0 + k >= h1) break;
+            T *yr = y + (h0 + k) * p.y_sh + u * E;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const float t = a[2 * i] * c[i] - a[2 * i + 1] * s[i];
-                a[2 * i + 1] = a[2 * i] * s[i] + a[2 * i + 1] * c[i];
-                a[2 * i] = t;
+                float &a = HALVES ? v[k][0][i] : v[k][0][2 * i], &b = HALVES ? v[k][P - 1][i] : v[k][0][2 * i + 1];
+                const float t = a * c[i] - b * s[i];
+                b = a * s[i] + b * c[i];
+                a = t;
             }
-            Io::put(yr + u * E, a);
-        } else {
-            const int i = HALVES ? u : 2 * u, j = HALVES ? u + half : 2 * u + 1;
-            const float a = Io::get(xr + i), b = Io::get(xr + j);
-            Io::put(yr + i, a * c[0] - b * s[0]);
-            Io::put(yr + j, a * s[0] + b * c[0]);
+            Io::put(yr, v[k][0]);
+            if constexpr (HALVES) Io::put(yr + half, v[k][1]);
+        }
+    } else {
+        const int i = HALVES ? u : 2 * u, j = HALVES ? u + half : 2 * u + 1;
+        for (int h = h0; h < h1; ++h) {
+            const float a = Io::get(x + h * p.x_sh + i), b = Io::get(x + h * p.x_sh + j);
+            Io::put(y + h * p.y_sh + i, a * c[0] - b * s[0]);
+            Io::put(y + h * p.y_sh + j, a * s[0] + b * c[0]);
         }
     }
 }
