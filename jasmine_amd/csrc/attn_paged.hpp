@@ -13,7 +13,11 @@
 //
 // fp32 rows: q and p as three bf16 parts each (exact, split.hpp), and fp32 cache values too, so
 // that 3 or 6 products make fp32 accuracy.  8-bit codes are bf16 numbers exactly; a key's scale
-// multiplies its scores, a value's scale its weight.
+// multiplies its scores, a value's scale its weight.  bf16 rows: p as one bf16 number where the sum
+// of the weights can be taken of what was rounded (by a product with ones: a row that one key
+// dominates then loses nothing), and as two where it cannot (scaled weights) or where the products
+// are for nothing (few rows): one part alone left results 1.5 times as far from 64 bits as their own
+// rounding does.
 //
 // What the products cannot give (infinities, NaN, sums past fp32, values that masked keys hold: a
 // weight of 0 times NaN) ends in a result that is not finite; such a row is computed again by
@@ -410,7 +414,16 @@ __device__ __forceinline__ void p_planes(const float (&e)[8], bf16x8 (&pf)[NP])
         split8(e, a, b, c);
         pf[0] = as_bf16x8(a), pf[1] = as_bf16x8(b), pf[2] = as_bf16x8(c);
     } else {
-        pf[0] = bf16x8{(__bf16)e[0], (__bf16)e[1], (__bf16)e[2], (__bf16)e[3], (__bf16)e[4], (__bf16)e[5], (__bf16)e[6], (__bf16)e[7]};
+        float r[8];
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const __bf16 h = (__bf16)(k ? r[j] : e[j]);
+                pf[k][j] = h;
+                r[j] = e[j] - (float)h;  // exact
+            }
+        }
     }
 }
 
@@ -471,6 +484,7 @@ template <int D, int CK, typename T>
 __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_kernel(const PagedAttnArgs p)
 {
     constexpr int M = 16, CD = D / 32, EV = D / 16, NP = sizeof(T) == 4 ? 3 : 1, NK = CK == CK_F32 ? 3 : 1;
+    constexpr int PP = sizeof(T) == 4 ? 3 : 2;  // planes of P
     using KO = KOperand<D, CK>;
     using VO = VOperand<CK, EV>;
     constexpr int ES = cache_bytes<CK>, LD = D + 4;
@@ -628,8 +642,8 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
         if (EIGHT)
 #pragma unroll
             for (int j = 0; j < 8; ++j) e[j] *= vsc[j];
-        bf16x8 pf[NP];
-        p_planes<NP>(e, pf);
+        bf16x8 pf[PP];
+        p_planes<PP>(e, pf);
 #pragma unroll
         for (int i = 0; i < EV; ++i) {
             u32x4 pl[NK];
@@ -701,6 +715,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
     using VO = VOperand<CK, EV>;
     constexpr int ES = cache_bytes<CK>, LD = D + 4, RING = NK == 3 || (CK >= CK_I8 && NQ == 2) ? 2 : 4;  // (as many as registers leave room for)
     constexpr bool EIGHT = CK >= CK_I8, ONES = NP == 1 && !EIGHT;  // row sums as P^T times ones
+    constexpr int PP = NP == 3 ? 3 : EIGHT ? 2 : 1;                // planes of P
     static_assert(NW % NJ == 0 && KC > 0, "a block of 16 keys is staged by NW / NJ waves");
     __shared__ u32x4 Ks[NB][NK][NJ * CD * 64];
     __shared__ u32x4 Vs[NB][NK][NC * NM * 64];
@@ -878,7 +893,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
                 for (int r = 0; r < 4; ++r) vsc[j][r] = (valid >> (16 * j + 4 * g + r) & 1) ? vsc[j][r] : 0.f;
             }
         }
-        bf16x8 pf[NM][NQ][NP];
+        bf16x8 pf[NM][NQ][PP];
 #pragma unroll
         for (int a = 0; a < NQ; ++a) {
             if (valid != (BK == 64 ? ~0ull : 0xffffffffull) || kv0 + BK > first_end[a]) {
@@ -924,7 +939,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
                 if (EIGHT)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) e[r] *= vsc[2 * m][r], e[4 + r] *= vsc[2 * m + 1][r];
-                p_planes<NP>(e, pf[m][a]);
+                p_planes<PP>(e, pf[m][a]);
                 if (ONES) lacc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[m][a][0], lacc[a], 0, 0, 0);
             }
         }
