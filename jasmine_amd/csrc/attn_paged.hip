@@ -70,6 +70,7 @@ jas_status jas_attn_paged(const void *q, void *o, const jas_paged_kv *kv, int n,
     rc = batch_view(n, B, cu, lens, p.bt, "jas_attn_paged");
     if (rc != JAS_OK) return rc;
     JAS_CHECK(q && o, JAS_ERR_INVALID, "jas_attn_paged: null q or o");
+    JAS_CHECK(q != o, JAS_ERR_INVALID, "jas_attn_paged: o must not overlap q");
     JAS_CHECK(dtype == JAS_F32 || dtype == JAS_BF16, JAS_ERR_INVALID, "jas_attn_paged: rows are JAS_F32 or JAS_BF16");
     JAS_CHECK(dtype == JAS_F32 || kv->dtype != JAS_F32, JAS_ERR_INVALID, "jas_attn_paged: JAS_BF16 rows over a JAS_F32 cache");
     JAS_CHECK(H > 0 && H % kv->n_kv == 0, JAS_ERR_INVALID, "jas_attn_paged: H is a multiple of the cache's heads");

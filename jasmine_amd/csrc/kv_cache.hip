@@ -16,24 +16,23 @@ namespace jas {
 
 jas_status paged_view(const jas_paged_kv *kv, PagedView &v, const char *who)
 {
-    const std::string w = std::string(who) + ": ";
-    JAS_CHECK(kv, JAS_ERR_INVALID, w + "null cache");
-    JAS_CHECK(kv->d_k && kv->d_v && kv->d_table, JAS_ERR_INVALID, w + "null pool or table");
+    JAS_CHECK(kv, JAS_ERR_INVALID, std::string(who) + ": null cache");
+    JAS_CHECK(kv->d_k && kv->d_v && kv->d_table, JAS_ERR_INVALID, std::string(who) + ": null pool or table");
     JAS_CHECK(kv->dtype == JAS_F32 || kv->dtype == JAS_BF16 || dtype_eight(kv->dtype), JAS_ERR_INVALID,
-              w + "the cache holds JAS_F32, JAS_BF16, JAS_I8 or JAS_F8E4M3");
-    JAS_CHECK(!dtype_eight(kv->dtype) || (kv->d_k_scale && kv->d_v_scale), JAS_ERR_INVALID, w + "an 8-bit cache needs its scales");
-    JAS_CHECK(kv->dh == 32 || kv->dh == 64 || kv->dh == 128, JAS_ERR_INVALID, w + "dh is 32, 64 or 128");
+              std::string(who) + ": the cache holds JAS_F32, JAS_BF16, JAS_I8 or JAS_F8E4M3");
+    JAS_CHECK(!dtype_eight(kv->dtype) || (kv->d_k_scale && kv->d_v_scale), JAS_ERR_INVALID, std::string(who) + ": an 8-bit cache needs its scales");
+    JAS_CHECK(kv->dh == 32 || kv->dh == 64 || kv->dh == 128, JAS_ERR_INVALID, std::string(who) + ": dh is 32, 64 or 128");
     JAS_CHECK(kv->n_pages > 0 && kv->page_size > 0 && kv->n_kv > 0 && kv->max_pages > 0 && kv->table_stride >= 0, JAS_ERR_INVALID,
-              w + "n_pages, page_size, n_kv and max_pages are positive, table_stride is not negative");
-    JAS_CHECK(kv->page_size <= 1 << 20, JAS_ERR_INVALID, w + "pages of at most 2^20 tokens");
+              std::string(who) + ": n_pages, page_size, n_kv and max_pages are positive, table_stride is not negative");
+    JAS_CHECK(kv->page_size <= 1 << 20, JAS_ERR_INVALID, std::string(who) + ": pages of at most 2^20 tokens");
     const long es = (long)dtype_bytes(kv->dtype);
     JAS_CHECK(kv->page_stride >= 0 && kv->head_stride >= 0 && kv->tok_stride >= kv->dh, JAS_ERR_INVALID,
-              w + "strides are not negative, and tokens at least dh apart");
+              std::string(who) + ": strides are not negative, and tokens at least dh apart");
     JAS_CHECK(((uintptr_t)kv->d_k | (uintptr_t)kv->d_v) % 16 == 0 && kv->page_stride * es % 16 == 0 &&
                   kv->head_stride * es % 16 == 0 && kv->tok_stride * es % 16 == 0,
-              JAS_ERR_INVALID, w + "rows of the cache start on 16 bytes");
+              JAS_ERR_INVALID, std::string(who) + ": rows of the cache start on 16 bytes");
     JAS_CHECK(((uintptr_t)kv->d_table | (uintptr_t)kv->d_k_scale | (uintptr_t)kv->d_v_scale) % 4 == 0, JAS_ERR_INVALID,
-              w + "table and scales aligned to 4 bytes");
+              std::string(who) + ": table and scales aligned to 4 bytes");
     v.k = kv->d_k, v.v = kv->d_v, v.ks = kv->d_k_scale, v.vs = kv->d_v_scale, v.table = kv->d_table;
     v.page_stride = kv->page_stride, v.head_stride = kv->head_stride, v.tok_stride = kv->tok_stride;
     v.table_stride = kv->table_stride, v.n_pages = kv->n_pages, v.page_size = kv->page_size, v.n_kv = kv->n_kv;
@@ -45,10 +44,9 @@ jas_status paged_view(const jas_paged_kv *kv, PagedView &v, const char *who)
 
 jas_status batch_view(int n, int B, const int32_t *cu, const int32_t *lens, BatchView &v, const char *who)
 {
-    const std::string w = std::string(who) + ": ";
-    JAS_CHECK(n >= 0 && B >= 0, JAS_ERR_INVALID, w + "n and B are not negative");
-    JAS_CHECK(B == 0 || (cu && lens), JAS_ERR_INVALID, w + "null cu or lens");
-    JAS_CHECK(((uintptr_t)cu | (uintptr_t)lens) % 4 == 0, JAS_ERR_INVALID, w + "cu and lens aligned to 4 bytes");
+    JAS_CHECK(n >= 0 && B >= 0, JAS_ERR_INVALID, std::string(who) + ": n and B are not negative");
+    JAS_CHECK(B == 0 || (cu && lens), JAS_ERR_INVALID, std::string(who) + ": null cu or lens");
+    JAS_CHECK(((uintptr_t)cu | (uintptr_t)lens) % 4 == 0, JAS_ERR_INVALID, std::string(who) + ": cu and lens aligned to 4 bytes");
     v = BatchView{cu, lens, B, n};
     return JAS_OK;
 }
@@ -292,18 +290,17 @@ template <bool READ>
 static jas_status kv_move(const jas_paged_kv *kv, void *k, void *v, int n, int64_t st, int64_t sh, int B, const int32_t *cu,
                           const int32_t *lens, int dtype, jas_stream_t stream, const char *who)
 {
-    const std::string w = std::string(who) + ": ";
     KvArgs p;
     jas_status rc = paged_view(kv, p.kv, who);
     if (rc != JAS_OK) return rc;
     rc = batch_view(n, B, cu, lens, p.bt, who);
     if (rc != JAS_OK) return rc;
-    JAS_CHECK(dtype == JAS_F32 || dtype == JAS_BF16, JAS_ERR_INVALID, w + "rows are JAS_F32 or JAS_BF16");
-    JAS_CHECK(READ || (k && v), JAS_ERR_INVALID, w + "null keys or values");
+    JAS_CHECK(dtype == JAS_F32 || dtype == JAS_BF16, JAS_ERR_INVALID, std::string(who) + ": rows are JAS_F32 or JAS_BF16");
+    JAS_CHECK(READ || (k && v), JAS_ERR_INVALID, std::string(who) + ": null keys or values");
     const uintptr_t es = dtype_bytes(dtype);
-    JAS_CHECK(((uintptr_t)k | (uintptr_t)v) % es == 0, JAS_ERR_INVALID, w + "rows aligned to their elements");
+    JAS_CHECK(((uintptr_t)k | (uintptr_t)v) % es == 0, JAS_ERR_INVALID, std::string(who) + ": rows aligned to their elements");
     if (!n || !B || (!k && !v)) return JAS_OK;
-    JAS_CHECK((double)n * kv->n_kv * (kv->dh / 8) <= 256.0 * 2147483647.0, JAS_ERR_RANGE, w + "too many rows for one call");
+    JAS_CHECK((double)n * kv->n_kv * (kv->dh / 8) <= 256.0 * 2147483647.0, JAS_ERR_RANGE, std::string(who) + ": too many rows for one call");
     p.x[0] = k, p.x[1] = v, p.st = st, p.sh = sh;
     p.vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (st * (long)es) % 16 == 0 && (sh * (long)es) % 16 == 0;
     hipStream_t s = stream_or_default(stream);

@@ -895,6 +895,8 @@ jas_status jas_sample(const void *x, int n, int V, int64_t ld, const float *temp
     JAS_CHECK(n >= 0 && V > 0 && V <= 1 << 22 && ld >= V, JAS_ERR_INVALID, "jas_sample: need n >= 0, V of 1 to 2^22 and ld >= V");
     JAS_CHECK(dtype == JAS_F32 || dtype == JAS_BF16, JAS_ERR_INVALID, "jas_sample: logits are JAS_F32 or JAS_BF16");
     JAS_CHECK((uintptr_t)x % (dtype == JAS_F32 ? 4 : 2) == 0, JAS_ERR_INVALID, "jas_sample: logits aligned to their elements");
+    JAS_CHECK(((uintptr_t)temp | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)u | (uintptr_t)ids | (uintptr_t)logp) % 4 == 0,
+              JAS_ERR_INVALID, "jas_sample: rows' values aligned to 4 bytes");
     if (!n) return JAS_OK;
     JAS_CHECK(n <= 65535, JAS_ERR_INVALID, "jas_sample: at most 65535 rows");
     JAS_CHECK(work && (uintptr_t)work % 16 == 0, JAS_ERR_INVALID, "jas_sample: need a workspace aligned to 16 bytes");

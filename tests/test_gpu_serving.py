@@ -359,6 +359,8 @@ def test_attention_long(jas, dtype, cache, news, lens):
     o, mag, big = R.attention(c, q, cu, lens, 0.125, 1, len(q))
     y = attend(jas, c, q, cu, lens, 0.125, 1, dtype)
     within(y, o, tolerance(o, mag, big, 64, max(lens), dtype))
+    if dtype == BF16 and max(news) <= 9 and cache != BF16:  # (weights of more than one bf16 part: the result's own rounding is left)
+        within(y, o, tolerance(o, mag, big, 64, max(lens), F32) + 2.0 ** -15 * mag + 2.0 ** -8 * np.abs(o))
     # the hosts' numbers only bound: a larger max_len and max_q give the same result
     y2 = attend(jas, c, q, cu, lens, 0.125, 1, dtype, max_q=int(max(news)) + 100, max_len=20000)
     within(y2, o, tolerance(o, mag, big, 64, max(lens), dtype))
@@ -507,6 +509,41 @@ def test_sample(jas, dtype, V, k, p, mp):
     x[1] = np.round(x[1])  # ties
     temp = rng.uniform(0.3, 1.5, n)
     check_draw(jas, x, dtype, temp, [k] * n, [p] * n, [mp] * n, rng.random(n), ld=V + 3 if V != 1000 else None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,ld", [(1, 200003, None), (2, 1200000, 1200001), (600, 17000, 17003), (1100, 2500, None), (40, 33000, 33008)])
+def test_sample_sizes(jas, dtype, n, V, ld):
+    """Rows of many chunks and many rows of few; starts off 16 bytes."""
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((min(n, 24), V)).astype(np.float32) * 2.5
+    x = x[np.arange(n) % len(x)]
+    for k, p, mp in ((0, 0.95, 0.0), (30, 0.9, 0.0), (0, 1.0, 0.03)):
+        rows = np.unique(np.concatenate([[0, n - 1], rng.integers(0, n, 8)]))
+        u = rng.random(n).astype(np.float32)
+        temp = rng.uniform(0.5, 1.2, n).astype(np.float32)
+        ids, lp = draw(jas, x, dtype, temp, [k] * n, [p] * n, [mp] * n, u, ld)
+        for i in rows:
+            want = R.sample(rounded(x[i], dtype), float(temp[i]), k, float(np.float32(p)), float(np.float32(mp)), float(u[i]))
+            assert ids[i] == want[0], (i, ids[i], want)
+            assert abs(lp[i] - want[1]) <= 2.0 ** -24 * abs(want[1]) + V * 2.0 ** -41 + 1e-13
+
+
+@pytest.mark.parametrize("V,k,p", [(50257, 2000, 1.0), (50257, 5000, 0.9), (6000, 5999, 0.5), (50257, 1024, 0.99), (50257, 1025, 0.99)])
+def test_sample_large_top_k(jas, V, k, p):
+    rng = np.random.default_rng(k)
+    check_draw(jas, rng.standard_normal((3, V)) * 3, F32, [0.9, 1.0, 5.0], [k] * 3, [p] * 3, None, rng.random(3))
+
+
+@pytest.mark.parametrize("spread", [1e-6, 1e-3, 100.0, 1e30])
+def test_sample_spreads(jas, spread):
+    """Logits all but equal, and ones whose weights are nearly all nothing; temperatures to match; a masked vocabulary."""
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((4, 30000)) * spread
+    x[3, 10:] = np.finfo(np.float32).min
+    for temp in (spread, spread * 0.01, 1.0, 1e-30):
+        for k, p, mp in ((0, 0.9, 0.0), (50, 1.0, 0.0), (0, 1.0, 0.2), (20, 0.5, 0.5)):
+            check_draw(jas, x, F32, [temp] * 4, [k] * 4, [p] * 4, [mp] * 4, rng.random(4))
 
 
 @pytest.mark.parametrize("V", [37, 8200])
@@ -682,6 +719,49 @@ def test_serving_two_streams(jas):
             x.check(*case)
     for st in streams:
         hip("hipStreamDestroy", st)
+
+
+@pytest.mark.parametrize("B", [300, 700])
+def test_attention_many_sequences(jas, B):
+    """More sequences than a workgroup has threads: short ones, some without new tokens, some longer."""
+    rng = np.random.default_rng(B)
+    news = rng.integers(0, 2, B)
+    news[[3, 7, B - 1]] = [40, 33, 20]
+    lens = news + rng.integers(0, 40, B)
+    c, cu, lens = filled(jas, rng, BF16, list(news), list(lens), 8, 1, 32)
+    for dtype in (F32, BF16):
+        q = rounded(rng.standard_normal((int(cu[-1]), 3, 32)), dtype)
+        o, mag, big = R.attention(c, q, cu, lens, 0.2, 1, len(q))
+        for max_q in (1, 40):
+            within(attend(jas, c, q, cu, lens, 0.2, 1, dtype, max_q=max_q), o, tolerance(o, mag, big, 32, 80, dtype))
+
+
+def test_far_slots(jas):
+    """A pool whose last pages lie past 2^31 elements: offsets of 64 bits."""
+    rng = np.random.default_rng(41)
+    heads, page, dh = 2, 16, 128
+    row = heads * page * dh
+    pages = (1 << 31) // row + 8
+    table = np.array([[pages - 1, 0, pages - 3, pages // 2 + 1, pages - 5]], np.int32)
+    pools = [jas.DeviceArray(pages * row, np.uint8) for _ in range(2)]
+    scales = [jas.DeviceArray(pages * heads * page, np.float32) for _ in range(2)]
+    d_table = jas.to_device(table)
+    kv = jas.PagedKv(pools[0].ptr, pools[1].ptr, scales[0].ptr, scales[1].ptr, d_table.ptr, row, page * dh, dh, 5, 5, F8, pages, page, heads, dh)
+    small = R.Cache(jas, F8, 5, heads, page, dh, np.arange(5, dtype=np.int32)[None])  # the plain copy: the same pages, near
+    L = 77
+    k, v = rng.standard_normal((2, L, heads, dh)).astype(np.float32)
+    whole, lens = np.array([0, L], np.int32), np.array([L], np.int32)
+    d_w, d_l, d_k, d_v = (jas.to_device(a) for a in (whole, lens, k, v))
+    jas.check(jas.lib.jas_kv_append(R.C.byref(kv), d_k.p, d_v.p, L, heads * dh, dh, 1, d_w.p, d_l.p, F32, None))
+    small.put(k, v, whole, lens)
+    for new in (1, 30):
+        cu = np.array([0, new], np.int32)
+        q = rounded(rng.standard_normal((new, 4, dh)), BF16)
+        o, mag, big = R.attention(small, q, cu, lens, 0.09, 1, new)
+        small.view, keep = kv, small.view
+        y = attend(jas, small, q, cu, lens, 0.09, 1, BF16)
+        small.view = keep
+        within(y, o, tolerance(o, mag, big, dh, L, BF16))
 
 
 def test_results_repeat(jas):

@@ -67,20 +67,21 @@ def test_kv_null_rows(capi):
 
 
 @pytest.mark.parametrize("kw,word,code", [
-    (dict(q=None), "null", 1), (dict(o=None), "null", 1), (dict(dtype=1), "rows are", 1), (dict(dtype=3), "over a JAS_F32 cache", 1),
+    (dict(q=None), "null", 1), (dict(o=None), "null", 1), (dict(o=P), "overlap", 1), (dict(work=P + 8), "16 bytes", 1),
+    (dict(work=None, max_len=100000), "workspace", 1), (dict(dtype=1), "rows are", 1), (dict(dtype=3), "over a JAS_F32 cache", 1),
     (dict(H=12), "multiple", 1), (dict(H=0), "multiple", 1), (dict(max_q=-1), "max_q", 1), (dict(max_len=-1), "max_q", 1),
     (dict(q=P + 2), "aligned", 1), (dict(n=1 << 28, H=16), "too many", 5)])
 def test_attention_refused(capi, kw, word, code):
-    v = dict(q=P, o=P, n=1, H=8, max_q=1, max_len=16, dtype=0)
+    v = dict(q=P, o=P + 4096, n=1, H=8, max_q=1, max_len=16, dtype=0, work=P)
     v.update(kw)
     refused(capi, capi.lib.jas_attn_paged(v["q"], v["o"], cache(capi), v["n"], 1, P, P, v["H"], v["max_q"], v["max_len"], 512, 64, 512, 64,
-                                          1.0, 1, v["dtype"], P, None), word, code)
+                                          1.0, 1, v["dtype"], v["work"], None), word, code)
 
 
 def test_attention_nothing_to_do(capi):
     args = (8, 1, 16, 512, 64, 512, 64, 1.0, 1, 0, None, None)
-    assert capi.lib.jas_attn_paged(P, P, cache(capi), 0, 1, P, P, *args) == 0
-    assert capi.lib.jas_attn_paged(P, P, cache(capi), 3, 0, None, None, *args) == 0
+    assert capi.lib.jas_attn_paged(P, P + 4096, cache(capi), 0, 1, P, P, *args) == 0
+    assert capi.lib.jas_attn_paged(P, P + 4096, cache(capi), 3, 0, None, None, *args) == 0
 
 
 @pytest.mark.parametrize("kw,word", [
@@ -96,13 +97,22 @@ def test_rope_refused(capi, kw, word):
 
 @pytest.mark.parametrize("kw,word", [
     (dict(x=None), "null"), (dict(u=None), "null"), (dict(ids=None), "null"), (dict(n=-1), "need n"), (dict(V=0), "need n"),
-    (dict(V=(1 << 22) + 1), "need n"), (dict(ld=9), "need n"), (dict(dtype=1), "logits are"), (dict(x=P + 2), "aligned")])
+    (dict(V=(1 << 22) + 1), "need n"), (dict(ld=9), "need n"), (dict(dtype=1), "logits are"), (dict(x=P + 2), "aligned"),
+    (dict(u=P + 2), "aligned"), (dict(n=65536), "65535"), (dict(work=None), "workspace"), (dict(work=P + 4), "workspace")])
 def test_sample_refused(capi, kw, word):
-    v = dict(x=P, n=1, V=10, ld=10, u=P, ids=P, dtype=0)
+    v = dict(x=P, n=1, V=10, ld=10, u=P, ids=P, dtype=0, work=P)
     v.update(kw)
     if v["V"] > 10:
         v["ld"] = v["V"]
-    refused(capi, capi.lib.jas_sample(v["x"], v["n"], v["V"], v["ld"], P, P, P, P, v["u"], v["ids"], P, v["dtype"], P, None), word)
+    refused(capi, capi.lib.jas_sample(v["x"], v["n"], v["V"], v["ld"], P, P, P, P, v["u"], v["ids"], P, v["dtype"], v["work"], None), word)
+
+
+def test_workspaces(capi):
+    """0 for what the calls refuse or return from at once, and no less for larger bounds."""
+    f, g = capi.lib.jas_attn_paged_workspace, capi.lib.jas_sample_workspace
+    assert f(0, 1, 8, 8, 64, 1, 16) == f(4, 0, 8, 8, 64, 1, 16) == f(4, 1, 8, 3, 64, 1, 16) == f(4, 1, 8, 8, 64, -1, 16) == 0
+    assert f(4, 4, 32, 8, 128, 1, 1 << 20) > 0 and g(0, 100) == g(1, 0) == g(1, (1 << 22) + 1) == 0
+    assert all(g(n, V) >= n * 8 for n in (1, 7, 3000) for V in (1, 5000, 1 << 22))
 
 
 # ---------------------------------------------------------------- frequencies
