@@ -27,16 +27,17 @@ static PagedPlan paged_plan(int n, int B, int H, int n_kv, int D, int max_q, int
     // Splits of `chunk` keys: enough workgroups to fill the chip some times over, so that sequences of
     // different lengths even out; a split that a shorter sequence does not need ends at once.
     const long full = std::min((long)r.tiles, std::max((long)B, (long)n * G / r.rows)) * n_kv, cus = paged_cus();
-    // Tiles of 16 rows: twelve rounds of one workgroup a unit (32 sequences of 1024 to 4096 keys, 8
-    // heads, bf16: 81.6, 75.5, 72.4, 81.6 us at 4, 8, 12, 16).  Larger tiles are bound by the matrix
+    // Tiles of 16 rows: eight rounds of one workgroup a unit (32 sequences of 1024 to 4096 keys, 8
+    // heads, bf16: 75.2, 71.0, 72.1, 78.9 us at 6, 8, 12, 16).  Larger tiles are bound by the matrix
     // cores and their partial results are large: split only where units would be left without one
     // (2 x 333 rows over 2001 keys, 12 heads of 64, fp32: 47.5, 38.7 us unsplit and at 3 rounds;
-    // 4 chunks of 512 over 4096, bf16: 143, 214).
+    // 4 chunks of 512 over 4096, bf16: 125, 163).  An odd number of splits: see paged_block.
     const bool few = r.rows > 16;
     if (few && full >= cus) r.chunk = std::max(max_len, 1), r.nsplit = 1;
     else {
-        r.chunk = (int)((std::max(few ? 256L : 128L, full * max_len / ((few ? 3 : 12) * cus)) + 127) / 128 * 128);
-        r.nsplit = (int)std::max(1L, std::min(((long)max_len + r.chunk - 1) / r.chunk, 64L));
+        r.chunk = (int)((std::max(few ? 256L : 128L, full * max_len / ((few ? 3 : 8) * cus)) + 127) / 128 * 128);
+        r.nsplit = (int)std::max(1L, std::min(((long)max_len + r.chunk - 1) / r.chunk, 63L));
+        if (r.nsplit > 1) r.nsplit |= 1;
     }
     return r;
 }

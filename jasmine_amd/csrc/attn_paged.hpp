@@ -139,6 +139,16 @@ __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, 
     return s_seq[3];
 }
 
+// A workgroup's key head, tile and split.  Key heads are the fastest: where they are a multiple of 8,
+// their tiles share one XCD's L2.  An XCD hands its workgroups to its shader engines in turn, so
+// nsplit is odd (paged_plan): with an even one every sequence's last splits, which shorter sequences
+// leave empty, would fall on the same engines.
+__device__ __forceinline__ void paged_block(const PagedAttnArgs &p, int &hk, int &x, int &split)
+{
+    const int id = blockIdx.x, rest = id / p.kv.n_kv;
+    hk = id % p.kv.n_kv, split = rest % p.nsplit, x = rest / p.nsplit;
+}
+
 // Keys [k_lo, k_hi) of a split: p.chunk of them, or as many as nsplit splits need to cover kend
 __device__ __forceinline__ void paged_split(const PagedAttnArgs &p, int kend, int split, int &k_lo, int &k_hi)
 {
@@ -496,7 +506,8 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
     __shared__ float s_sc[4][2][32];
     const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int hk = blockIdx.x % p.kv.n_kv, rest = blockIdx.x / p.kv.n_kv, split = rest % p.nsplit, x = rest / p.nsplit;
+    int hk, x, split;
+    paged_block(p, hk, x, split);
     int b;
     PagedSeq sq;
     const int tile = paged_tile<M, 256>(p, x, b, sq);
@@ -725,7 +736,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
     __shared__ unsigned s_bad[4];
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x % p.kv.n_kv, rest = blockIdx.x / p.kv.n_kv, split = rest % p.nsplit, x = rest / p.nsplit;
+    int hk, x, split;
+    paged_block(p, hk, x, split);
     int b;
     PagedSeq sq;
     const int tile = p.sorted ? paged_tile_sorted<M>(p, x, b, sq) : paged_tile<M, 64 * NW>(p, x, b, sq);
