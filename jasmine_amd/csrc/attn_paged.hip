@@ -20,13 +20,14 @@ static int paged_cus()
 static PagedPlan paged_plan(int n, int B, int H, int n_kv, int D, int max_q, int max_len, int dtype)
 {
     PagedPlan r;
+    max_len = std::min(max_len, 0x7fff0000);  // (no table's row holds more: PagedView)
     const long G = H / n_kv, most = std::min((long)max_q, (long)n) * G;
     r.rows = most <= 16 ? 16 : most <= 64 || (dtype == JAS_F32 && D == 128) ? 64 : 128;
     // sequence b owns tiles from floor(cu[b] G / rows) + b on
-    r.tiles = (int)((long)n * G / r.rows + B);
+    r.tiles = (long)n * G / r.rows + B;
     // Splits of `chunk` keys: enough workgroups to fill the chip some times over, so that sequences of
     // different lengths even out; a split that a shorter sequence does not need ends at once.
-    const long full = std::min((long)r.tiles, std::max((long)B, (long)n * G / r.rows)) * n_kv, cus = paged_cus();
+    const long full = std::min(r.tiles, std::max((long)B, (long)n * G / r.rows)) * n_kv, cus = paged_cus();
     // Tiles of 16 rows: eight rounds of one workgroup a unit (32 sequences of 1024 to 4096 keys, 8
     // heads, bf16: 75.2, 71.0, 72.1, 78.9 us at 6, 8, 12, 16).  Larger tiles are bound by the matrix
     // cores and their partial results are large: split only where units would be left without one
@@ -35,7 +36,8 @@ static PagedPlan paged_plan(int n, int B, int H, int n_kv, int D, int max_q, int
     const bool few = r.rows > 16;
     if (few && full >= cus) r.chunk = std::max(max_len, 1), r.nsplit = 1;
     else {
-        r.chunk = (int)((std::max(few ? 256L : 128L, full * max_len / ((few ? 3 : 8) * cus)) + 127) / 128 * 128);
+        const double share = (double)full * max_len / ((few ? 3 : 8) * cus);
+        r.chunk = (int)std::min(((long)std::max(few ? 256.0 : 128.0, std::min(share, (double)max_len)) + 127) / 128 * 128, 0x7fff0000L);
         r.nsplit = (int)std::max(1L, std::min(((long)max_len + r.chunk - 1) / r.chunk, 63L));
         if (r.nsplit > 1) r.nsplit |= 1;
     }
@@ -81,7 +83,8 @@ jas_status jas_attn_paged(const void *q, void *o, const jas_paged_kv *kv, int n,
     JAS_CHECK((long)n * H <= 0x3fffffffl, JAS_ERR_RANGE, "jas_attn_paged: too many rows for one call");
     if (!n || !B) return JAS_OK;
     const PagedPlan plan = paged_plan(n, B, H, kv->n_kv, kv->dh, max_q, max_len, dtype);
-    JAS_CHECK((double)plan.tiles * kv->n_kv * std::max(plan.nsplit, plan.rows / 4) <= 2147483647.0, JAS_ERR_RANGE, "jas_attn_paged: too many tiles for one call");
+    // (a launch holds less than 2^32 threads: up to 512 of a tile, 256 of four rows that are joined)
+    JAS_CHECK((double)plan.tiles * kv->n_kv * std::max(plan.nsplit, plan.nsplit > 1 ? plan.rows / 4 : 1) <= 8388607.0, JAS_ERR_RANGE, "jas_attn_paged: too many tiles for one call");
     JAS_CHECK(plan.nsplit == 1 || work, JAS_ERR_INVALID, "jas_attn_paged: null workspace");
     JAS_CHECK((uintptr_t)work % 16 == 0, JAS_ERR_INVALID, "jas_attn_paged: workspace aligned to 16 bytes");
     p.q = q, p.o = o, p.H = H, p.G = H / kv->n_kv, p.max_len = max_len, p.causal = causal != 0;
@@ -90,7 +93,7 @@ jas_status jas_attn_paged(const void *q, void *o, const jas_paged_kv *kv, int n,
     p.q_vec = (uintptr_t)q % 16 == 0 && q_st * es % 16 == 0 && q_sh * es % 16 == 0;
     p.o_vec = (uintptr_t)o % 16 == 0 && o_st * es % 16 == 0 && o_sh * es % 16 == 0;
     p.scale_log2 = scale * 1.44269504088896340736f;
-    p.tiles = plan.tiles, p.nsplit = plan.nsplit, p.chunk = plan.chunk, p.sorted = plan.rows > 16 && plan.nsplit == 1 && B <= 256, p.cus = paged_cus(), p.part = (float *)work;
+    p.tiles = (int)plan.tiles, p.nsplit = plan.nsplit, p.chunk = plan.chunk, p.sorted = plan.rows > 16 && plan.nsplit == 1 && B <= 256, p.cus = paged_cus(), p.part = (float *)work;
     hipStream_t s = stream_or_default(stream);
     if (kv->dh == 32) paged_launch_32(p, plan.rows, kv->dtype, dtype, s);
     else if (kv->dh == 64) paged_launch_64(p, plan.rows, kv->dtype, dtype, s);

@@ -48,7 +48,8 @@ struct PagedAttnArgs {
 // How a call is launched
 struct PagedPlan {
     int rows;  // of a tile: 16 (its waves share the keys), 64 or 128
-    int tiles, nsplit, chunk;
+    long tiles;
+    int nsplit, chunk;
 };
 // One call's kernels for head dim 32, 64, 128
 void paged_launch_32(const PagedAttnArgs &p, int rows, int cache, int dtype, hipStream_t s);
@@ -154,7 +155,7 @@ __device__ __forceinline__ void paged_split(const PagedAttnArgs &p, int kend, in
 {
     const int per = max(p.chunk, ((kend + p.nsplit - 1) / p.nsplit + 127) / 128 * 128);
     k_lo = (int)min((long)kend, (long)split * per);
-    k_hi = min(kend, k_lo + per);
+    k_hi = (int)min((long)kend, (long)k_lo + per);
 }
 
 // Where key t of sequence b lies: the table's entry for its page, and the slot

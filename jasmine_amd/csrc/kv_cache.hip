@@ -300,7 +300,8 @@ static jas_status kv_move(const jas_paged_kv *kv, void *k, void *v, int n, int64
     const uintptr_t es = dtype_bytes(dtype);
     JAS_CHECK(((uintptr_t)k | (uintptr_t)v) % es == 0, JAS_ERR_INVALID, std::string(who) + ": rows aligned to their elements");
     if (!n || !B || (!k && !v)) return JAS_OK;
-    JAS_CHECK((double)n * kv->n_kv * (kv->dh / 8) <= 256.0 * 2147483647.0, JAS_ERR_RANGE, std::string(who) + ": too many rows for one call");
+    // (a launch holds less than 2^32 threads)
+    JAS_CHECK((double)n * kv->n_kv * (kv->dh / 8) * (READ ? 1 : 2) <= 4294966784.0, JAS_ERR_RANGE, std::string(who) + ": too many rows for one call");
     p.x[0] = k, p.x[1] = v, p.st = st, p.sh = sh;
     p.vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (st * (long)es) % 16 == 0 && (sh * (long)es) % 16 == 0;
     hipStream_t s = stream_or_default(stream);

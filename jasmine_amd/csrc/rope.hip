@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs p)
 }
 
 template <typename T>
-static void rope_launch(RopeArgs &p, int layout, hipStream_t s)
+static jas_status rope_launch(RopeArgs &p, int layout, hipStream_t s)
 {
     constexpr int E = RopeIo<T>::E;
     const bool halves = layout == JAS_ROPE_HALVES;
@@ -153,11 +153,15 @@ static void rope_launch(RopeArgs &p, int layout, hipStream_t s)
     const int pairs = vec ? (halves ? E : E / 2) : 1;
     p.units = p.rot / 2 / pairs + (p.dh - p.rot) / (vec ? E : 1);
     p.groups = (p.nh + ROPE_HEADS - 1) / ROPE_HEADS;
+    // (a launch holds less than 2^32 threads)
+    JAS_CHECK((double)p.n * p.units * p.groups <= 4294967040.0, JAS_ERR_RANGE, "jas_rope: too many elements for one call");
     const dim3 grid(ceil_div((long)p.n * p.units * p.groups, 256)), block(256);
     if (halves && vec) hipLaunchKernelGGL((rope_kernel<T, true, true>), grid, block, 0, s, p);
     else if (halves) hipLaunchKernelGGL((rope_kernel<T, true, false>), grid, block, 0, s, p);
     else if (vec) hipLaunchKernelGGL((rope_kernel<T, false, true>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((rope_kernel<T, false, false>), grid, block, 0, s, p);
+    JAS_LAUNCH_CHECK();
+    return JAS_OK;
 }
 
 } // namespace jas
@@ -179,13 +183,8 @@ jas_status jas_rope(const void *x, void *y, const int32_t *pos, const double *fr
     JAS_CHECK((uintptr_t)freq % 8 == 0 && (uintptr_t)pos % 4 == 0 && ((uintptr_t)x | (uintptr_t)y) % (dtype == JAS_F32 ? 4 : 2) == 0,
               JAS_ERR_INVALID, "jas_rope: pointers aligned to their elements");
     if (!n) return JAS_OK;
-    // one thread for each element at most: the grid has to hold them
-    JAS_CHECK((double)n * nh * dh <= 256.0 * 2147483647.0, JAS_ERR_RANGE, "jas_rope: too many elements for one call");
     RopeArgs p{x, y, pos, freq, n, nh, dh, rot, (long)x_st, (long)x_sh, (long)y_st, (long)y_sh, mscale, 0, 0};
-    if (dtype == JAS_F32) rope_launch<float>(p, layout, stream_or_default(stream));
-    else rope_launch<uint16_t>(p, layout, stream_or_default(stream));
-    JAS_LAUNCH_CHECK();
-    return JAS_OK;
+    return dtype == JAS_F32 ? rope_launch<float>(p, layout, stream_or_default(stream)) : rope_launch<uint16_t>(p, layout, stream_or_default(stream));
 }
 
 jas_status jas_rope_freqs(int rot, double theta, const jas_rope_scaling *sc, double *h_freq, float *h_mscale)

@@ -366,6 +366,16 @@ def test_attention_long(jas, dtype, cache, news, lens):
     within(y2, o, tolerance(o, mag, big, 64, max(lens), dtype))
 
 
+@pytest.mark.parametrize("news,lens", [([1, 1], [700, 5]), ([20, 3], [300, 900]), ([40], [41])])
+def test_attention_any_bound(jas, news, lens):
+    """The largest max_len there is: the results are within the same tolerance."""
+    rng = np.random.default_rng(20)
+    c, cu, lens = filled(jas, rng, BF16, news, lens, 16, 2, 64)
+    q = rng.standard_normal((int(cu[-1]), 6, 64)).astype(np.float32)
+    o, mag, big = R.attention(c, q, cu, lens, 0.125, 1, len(q))
+    within(attend(jas, c, q, cu, lens, 0.125, 1, F32, max_len=2 ** 31 - 1), o, tolerance(o, mag, big, 64, max(lens), F32))
+
+
 @pytest.mark.parametrize("dtype,cache", [(F32, F32), (BF16, BF16), (F32, F8)])
 def test_attention_empty_and_outside(jas, dtype, cache):
     """Sequences of no token, lengths below the new tokens, above max_len and above the table's row,

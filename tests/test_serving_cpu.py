@@ -115,6 +115,23 @@ def test_workspaces(capi):
     assert all(g(n, V) >= n * 8 for n in (1, 7, 3000) for V in (1, 5000, 1 << 22))
 
 
+@pytest.mark.parametrize("n,B,H,n_kv,max_q", [(512, 512, 64, 8, 1), (4, 4, 32, 8, 1), (1 << 20, 1 << 20, 64, 64, 1), (5, 1, 8, 8, 5), (64, 2, 32, 8, 32)])
+def test_workspace_of_any_bound(capi, n, B, H, n_kv, max_q):
+    """max_len only bounds: the largest one is as good as another, and 63 parts of a row are the most."""
+    for max_len in (0, 1, 4096, 1 << 24, 1 << 30, 2 ** 31 - 1):
+        size = capi.lib.jas_attn_paged_workspace(n, B, H, n_kv, 64, max_q, max_len)
+        assert 0 <= size <= (n * (H // n_kv) + 128 * B) * n_kv * 63 * (64 + 4) * 4
+
+
+def test_launches_that_would_not_fit(capi):
+    """2^32 threads or more in one launch are refused before it."""
+    big = 2 ** 31 - 1
+    refused(capi, capi.lib.jas_rope(P, P, P, P, big, 64, 64, 64, 4096, 64, 4096, 64, 0, 1.0, 0, None), "too many", 5)
+    for f in (capi.lib.jas_kv_append, capi.lib.jas_kv_read):
+        refused(capi, f(cache(capi), P, P, big, 512, 64, 1, P, P, 0, None), "too many", 5)
+    refused(capi, capi.lib.jas_attn_paged(P, P + 4096, cache(capi), 1 << 20, 1 << 23, P, P, 8, 1, 16, 512, 64, 512, 64, 1.0, 1, 0, P, None), "too many", 5)
+
+
 # ---------------------------------------------------------------- frequencies
 def freqs(capi, *a, **kw):
     return capi.rope_freqs(*a, **kw)
