@@ -109,8 +109,9 @@ __device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b,
 // The same in order of falling length, for launches whose workgroups own whole sequences of keys (B
 // <= 256): each thread adds the tiles of the sequences before its own.  Workgroups start in the order
 // of their ids; where two fit on a unit, i and i + cus share one, so the second cus of them are
-// taken from the light end (cus 0: they do not): 8 chunks of up to 256 beside 16 decoding sequences,
-// 148 -> 122 us.
+// taken from the light end (cus 0: they do not).  24 sequences of up to 2048 keys, chunks of up to 256
+// beside single tokens: e4m3 138 -> 121 us, bf16 96 -> 77; 4 chunks of up to 512 over up to 4096 keys, bf16:
+// 137 -> 126.
 template <int M>
 __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
 {
@@ -486,6 +487,9 @@ __device__ __forceinline__ void q_planes(const T *q, bool there, int g, bool vec
 // turn and keep a softmax each, joined at the end.  Nothing goes through LDS on the way: K and V
 // are read from memory in operand order (each 16-lane group reads whole value rows, 64-byte
 // pieces of key rows), V is transposed by v_perm in the lane that read it.
+// Bound by memory: 32 sequences of 1024 to 4096 keys, 8 heads of 128, bf16: 342 MB in 71.5 us with the
+// merge, 4.8 TB/s (a copy of 1 GiB: 5.1); 3 of up to 65536 in int8: 327 MB in 73; one of 1000 in fp32: 10 us,
+// two launches and a chain of dependent loads.
 // Waves a SIMD: loads in flight hide the memory's latency, as many as registers hold (fp32 rows keep
 // three planes of Q, fp32 caches twice the raw words)
 template <int D, int CK, typename T>
@@ -713,8 +717,13 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
 // Where operands are single bf16 planes two buffers of LDS need one barrier a tile; three planes
 // take one buffer and two barriers.
 // 32 rows a wave read a fragment from LDS for twice the products; 16 leave registers for more waves,
-// which share out the widening of codes: bf16 rows over 8-bit caches at D = 128 (4 chunks of 512 over
-// 4096 keys, int8: 234 us with 32, 175 with 16; over bf16 139 and 147).
+// which share out the widening of codes: bf16 rows over 8-bit caches at D = 128 (4 chunks of up to 512 over
+// up to 4096 keys, int8: 258 us with 32, 198 with 16; over bf16 126 and 132).
+// Those chunks over bf16 are 73.6 GFLOP: 587 TFLOP/s, where a large bf16 product of a library reaches 1208.
+// The matrix cores are busy 0.25 of the time that all units are held, the vector ALU (softmax, staging)
+// 0.32, one mostly while the other waits; the rest is two tiles a unit of unequal length.  Two groups of
+// waves that share a tile's keys (142 us), keys split so that tiles are equal (158), two sets of
+// registers for the staged rows (no change) and longer rings (they spill: 151) were slower.
 template <int D, int CK, typename T, int NQ, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnArgs p)
 {
@@ -1018,7 +1027,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
 }
 
 // Joins the splits of a tile's rows, one wave a row: lane i weighs split i (nsplit <= 64), then the
-// wave adds the means of the splits that have weight, sixteen in flight.
+// wave adds the means of the splits that have weight, sixteen in flight.  (6 us of the 71.5 above; 9 of
+// int8's 73, whose rows have 63 splits.)
 template <int D, typename T>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs p, int M)
 {

