@@ -83,8 +83,8 @@ jas_status jas_attn_paged(const void *q, void *o, const jas_paged_kv *kv, int n,
     JAS_CHECK((long)n * H <= 0x3fffffffl, JAS_ERR_RANGE, "jas_attn_paged: too many rows for one call");
     if (!n || !B) return JAS_OK;
     const PagedPlan plan = paged_plan(n, B, H, kv->n_kv, kv->dh, max_q, max_len, dtype);
-    // (a launch holds less than 2^32 threads: up to 512 of a tile, 256 of four rows that are joined)
-    JAS_CHECK((double)plan.tiles * kv->n_kv * std::max(plan.nsplit, plan.nsplit > 1 ? plan.rows / 4 : 1) <= 8388607.0, JAS_ERR_RANGE, "jas_attn_paged: too many tiles for one call");
+    // (a launch holds less than 2^32 threads: 256 of a tile, and of four rows that are joined)
+    JAS_CHECK((double)plan.tiles * kv->n_kv * std::max(plan.nsplit, plan.nsplit > 1 ? plan.rows / 4 : 1) <= 16777215.0, JAS_ERR_RANGE, "jas_attn_paged: too many tiles for one call");
     JAS_CHECK(plan.nsplit == 1 || work, JAS_ERR_INVALID, "jas_attn_paged: null workspace");
     JAS_CHECK((uintptr_t)work % 16 == 0, JAS_ERR_INVALID, "jas_attn_paged: workspace aligned to 16 bytes");
     p.q = q, p.o = o, p.H = H, p.G = H / kv->n_kv, p.max_len = max_len, p.causal = causal != 0;

@@ -41,7 +41,7 @@ struct PagedAttnArgs {
     float scale_log2;
     int q_vec, o_vec;           // rows of Q, O start on 16 bytes
     int tiles, nsplit, chunk;   // grid: tiles x nsplit x key heads; keys of a split, at least
-    int sorted, cus;            // tiles in order of falling length; compute units, if two tiles share one
+    int sorted, cus;            // tiles in order of falling length; compute units
     float *part;                // nsplit > 1: rows of D means, then exponent base and sum
 };
 
@@ -84,14 +84,14 @@ struct PagedSeq {
 // Tile x of the grid: sequence b owns tiles from floor(cu[b] G / M) + b on, at least as many as
 // its rows fill, so the thread that holds b knows it from cu[b] and cu[b + 1] alone: one round of
 // loads, no running sum.  Returns x's tile number in b, or -1.  By the whole workgroup.
-template <int M, int NT>
+template <int M>
 __device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
 {
     __shared__ int s_b, s_seq[4];
     if (threadIdx.x == 0) s_b = -1, s_seq[3] = -1;
     __syncthreads();
     int own = -2, row0 = 0, rows = 0, len = 0, at = 0;
-    for (int j = threadIdx.x; j < p.bt.B; j += NT) {
+    for (int j = threadIdx.x; j < p.bt.B; j += 256) {
         const int c0 = max(0, min(p.bt.cu[j], p.bt.n)), c1 = max(c0, min(p.bt.cu[j + 1], p.bt.n)), n = p.bt.lens[j];
         const int first = (int)((long)c0 * p.G / M + j);
         if (first <= x && (j + 1 == p.bt.B || (int)((long)c1 * p.G / M + j + 1) > x))
@@ -109,8 +109,8 @@ __device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b,
 // The same in order of falling length, for launches whose workgroups own whole sequences of keys (B
 // <= 256): each thread adds the tiles of the sequences before its own.  Workgroups start in the order
 // of their ids; where two fit on a unit, i and i + cus share one, so the second cus of them are
-// taken from the light end (cus 0: they do not).  24 sequences of up to 2048 keys, chunks of up to 256
-// beside single tokens: e4m3 138 -> 121 us, bf16 96 -> 77; 4 chunks of up to 512 over up to 4096 keys, bf16:
+// taken from the light end.  24 sequences of up to 2048 keys, chunks of up to 256
+// beside single tokens, bf16: 96 -> 77 us; 4 chunks of up to 512 over up to 4096 keys, bf16:
 // 137 -> 126.
 template <int M>
 __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
@@ -124,7 +124,7 @@ __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, 
         len = max(0, min(p.bt.lens[j], min(p.kv.cap, p.max_len)));
     }
     const int tiles = (int)(((long)rows * p.G + M - 1) / M);
-    if (j < 256) s_tiles[j] = tiles, s_len[j] = len;
+    s_tiles[j] = tiles, s_len[j] = len;
     if (j == 0) s_seq[3] = -1, s_seq[4] = 0;
     __syncthreads();
     int first = 0, total = 0;
@@ -257,12 +257,12 @@ __device__ __forceinline__ PagedRow paged_row_of(const PagedAttnArgs &p, const P
 }
 
 // Computes the rows of a tile again whose bit in bad[] is set: results or partial results
-template <int D, int CK, typename T, int NW>
+template <int D, int CK, typename T>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &p, int b, int hk, const PagedSeq &sq, int r0, int rows,
                                                       const unsigned *bad, int k_lo, int k_hi, float *part)
 {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int r = w; r < rows; r += NW) {
+    for (int r = w; r < rows; r += 4) {
         if (!(bad[r / 32] >> (r % 32) & 1)) continue;
         const PagedRow row = paged_row_of(p, sq, hk, r0 + r);
         float m, l, out[(D + 63) / 64];
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
     paged_block(p, hk, x, split);
     int b;
     PagedSeq sq;
-    const int tile = paged_tile<M, 256>(p, x, b, sq);
+    const int tile = paged_tile<M>(p, x, b, sq);
     const int r0 = tile * M, rows = min(M, sq.rows * p.G - r0);
     if (tile < 0 || rows <= 0) return;
     const PagedRow row = paged_row_of(p, sq, hk, r0 + min(r16, rows - 1));
@@ -707,34 +707,35 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
         }
     }
     if (part && w == 0 && g == 0 && r16 < rows && !(bad >> r16 & 1)) part[(long)r16 * LD + D] = mm, part[(long)r16 * LD + D + 1] = ll;
-    if (bad) paged_again<D, CK, T, 4>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
+    if (bad) paged_again<D, CK, T>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
 }
 
 // ---------------------------------------------------------------- many rows: chunks
-// One workgroup: a tile of 16 NQ NW rows, 16 NQ a wave of NW, and one split of its keys.  Tiles of BK keys go
+// One workgroup: a tile of 64 NQ rows, 16 NQ a wave, and one split of its keys.  Tiles of BK keys go
 // through LDS in operand order (one ds_read_b128 a fragment, no bank conflict on either side): read
 // from their pages a tile ahead, widened or split once, V transposed by the lanes that stage it.
 // Where operands are single bf16 planes two buffers of LDS need one barrier a tile; three planes
 // take one buffer and two barriers.
-// 32 rows a wave read a fragment from LDS for twice the products; 16 leave registers for more waves,
-// which share out the widening of codes: bf16 rows over 8-bit caches at D = 128 (4 chunks of up to 512 over
-// up to 4096 keys, int8: 258 us with 32, 198 with 16; over bf16 126 and 132).
+// 32 rows a wave read a fragment from LDS for twice the products that 16 do.  With 16 and eight waves, which
+// share out the staging, 4 chunks of up to 512 over up to 4096 keys take 181 us over int8 and 132 over bf16,
+// with 32 and four 171 and 126; with 32 and eight, tiles of 256 rows are too few to even out: 260.  Scales of
+// values are read from LDS where they are used: held in registers (two fragments in flight): 258.
 // Those chunks over bf16 are 73.6 GFLOP: 587 TFLOP/s, where a large bf16 product of a library reaches 1208.
 // The matrix cores are busy 0.25 of the time that all units are held, the vector ALU (softmax, staging)
 // 0.32, one mostly while the other waits; the rest is two tiles a unit of unequal length.  Two groups of
 // waves that share a tile's keys (142 us), keys split so that tiles are equal (158), two sets of
 // registers for the staged rows (no change) and longer rings (they spill: 151) were slower.
-template <int D, int CK, typename T, int NQ, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnArgs p)
+template <int D, int CK, typename T, int NQ>
+__global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs p)
 {
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, NK = CK == CK_F32 ? 3 : 1, NB = NK == 3 ? 1 : 2;
-    constexpr int BK = NK == 3 && D == 128 ? 32 : 64, M = 16 * NQ * NW;
+    constexpr int BK = NK == 3 && D == 128 ? 32 : 64, NW = 4, M = 16 * NQ * NW;
     constexpr int CD = D / 32, NC = D / 16, NJ = BK / 16, NM = BK / 32;
-    constexpr int EV = D == 128 && NW == 4 ? 4 : 2, NH = D / (16 * EV), NU = NM * NH;  // V: units of 32 keys x 16 EV d
+    constexpr int EV = D == 128 ? 4 : 2, NH = D / (16 * EV), NU = NM * NH;  // V: units of 32 keys x 16 EV d
     constexpr int KC = CD * NJ / NW;  // K: a wave stages KC steps of 16 keys
     using KO = KOperand<D, CK>;
     using VO = VOperand<CK, EV>;
-    constexpr int ES = cache_bytes<CK>, LD = D + 4, RING = NK == 3 || (CK >= CK_I8 && NQ == 2) ? 2 : 4;  // (as many as registers leave room for)
+    constexpr int ES = cache_bytes<CK>, LD = D + 4, RING = NK == 3 ? 2 : 4;  // (as many as registers leave room for)
     constexpr bool EIGHT = CK >= CK_I8, ONES = NP == 1 && !EIGHT;  // row sums as P^T times ones
     constexpr int PP = NP == 3 ? 3 : EIGHT ? 2 : 1;                // planes of P
     static_assert(NW % NJ == 0 && KC > 0, "a block of 16 keys is staged by NW / NJ waves");
@@ -750,7 +751,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
     paged_block(p, hk, x, split);
     int b;
     PagedSeq sq;
-    const int tile = p.sorted ? paged_tile_sorted<M>(p, x, b, sq) : paged_tile<M, 64 * NW>(p, x, b, sq);
+    const int tile = p.sorted ? paged_tile_sorted<M>(p, x, b, sq) : paged_tile<M>(p, x, b, sq);
     const int r0 = tile * M, rows = min(M, sq.rows * p.G - r0);
     if (tile < 0 || rows <= 0) return;
     const int kend = paged_row_of(p, sq, hk, r0 + rows - 1).end;  // (the last row of a tile sees most)
@@ -817,7 +818,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
         }
     };
     auto lstore = [&](int buf, int at, unsigned long long valid) {
-        if (EIGHT && w == 0) s_sc[at][0][lane] = ks, s_sc[at][1][lane] = vs;
+        if (EIGHT && w == 0) s_sc[at][0][lane] = ks, s_sc[at][1][lane] = (valid >> lane & 1) ? vs : 0.f;
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             u32x4 pl[NK];
@@ -903,16 +904,12 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
         }
 #pragma unroll
         for (int f = 0; f < RING - 1; ++f) fetch_v(f);
-        floatx4 vsc[NJ];
         if (EIGHT) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const floatx4 f = *(const floatx4 *)&s_sc[at][0][16 * j + 4 * g];
-                vsc[j] = *(const floatx4 *)&s_sc[at][1][16 * j + 4 * g];
 #pragma unroll
                 for (int a = 0; a < NQ; ++a) s[j][a] *= f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) vsc[j][r] = (valid >> (16 * j + 4 * g + r) & 1) ? vsc[j][r] : 0.f;
             }
         }
         bf16x8 pf[NM][NQ][PP];
@@ -958,9 +955,11 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
 #pragma unroll
                 for (int r = 0; r < 4; ++r) e[r] = paged_exp2(s[2 * m][a][r]), e[4 + r] = paged_exp2(s[2 * m + 1][a][r]);
                 if (!ONES) l[a] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                if (EIGHT)
+                if (EIGHT) {
+                    const floatx4 v0 = *(const floatx4 *)&s_sc[at][1][32 * m + 4 * g], v1 = *(const floatx4 *)&s_sc[at][1][32 * m + 16 + 4 * g];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) e[r] *= vsc[2 * m][r], e[4 + r] *= vsc[2 * m + 1][r];
+                    for (int r = 0; r < 4; ++r) e[r] *= v0[r], e[4 + r] *= v1[r];
+                }
                 p_planes<PP>(e, pf[m][a]);
                 if (ONES) lacc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[m][a][0], lacc[a], 0, 0, 0);
             }
@@ -1023,7 +1022,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttnA
         if (part && g == 0) part[(long)r * LD + D] = ll != 0.f ? mb[a] : -INFINITY, part[(long)r * LD + D + 1] = ll;
     }
     __syncthreads();
-    if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) paged_again<D, CK, T, NW>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
+    if (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) paged_again<D, CK, T>(p, b, hk, sq, r0, rows, s_bad, k_lo, k_hi, part);
 }
 
 // Joins the splits of a tile's rows, one wave a row: lane i weighs split i (nsplit <= 64), then the
@@ -1037,7 +1036,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs p,
     const int quarter = blockIdx.x % (M / 4), rest = blockIdx.x / (M / 4), hk = rest % p.kv.n_kv, x = rest / p.kv.n_kv;
     int b;
     PagedSeq sq;
-    const int tile = M == 16 ? paged_tile<16, 256>(p, x, b, sq) : M == 64 ? paged_tile<64, 256>(p, x, b, sq) : paged_tile<128, 256>(p, x, b, sq);
+    const int tile = M == 16 ? paged_tile<16>(p, x, b, sq) : M == 64 ? paged_tile<64>(p, x, b, sq) : paged_tile<128>(p, x, b, sq);
     const int r = quarter * 4 + w;
     if (tile < 0 || r >= sq.rows * p.G - tile * M) return;
     const float *part = p.part + (((long)x * p.kv.n_kv + hk) * p.nsplit * M + r) * LD;
@@ -1079,12 +1078,8 @@ void paged_launch_as(const PagedAttnArgs &p, int rows, hipStream_t s)
 {
     const dim3 grid((unsigned)p.tiles * p.nsplit * p.kv.n_kv), block(256);
     if (rows == 16) hipLaunchKernelGGL((paged_stream_kernel<D, CK, T>), grid, block, 0, s, p);
-    else if (rows == 64) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1, 4>), grid, block, 0, s, p);
-    else if constexpr (D == 128 && CK >= CK_I8 && sizeof(T) == 2) {
-        PagedAttnArgs one = p;
-        one.cus = 0;  // (one workgroup a unit)
-        hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1, 8>), grid, dim3(512), 0, s, one);
-    } else if constexpr (sizeof(T) == 2 || D < 128) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 2, 4>), grid, block, 0, s, p);
+    else if (rows == 64) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1>), grid, block, 0, s, p);
+    else if constexpr (sizeof(T) == 2 || D < 128) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 2>), grid, block, 0, s, p);
     if (p.nsplit > 1) hipLaunchKernelGGL((paged_merge_kernel<D, T>), dim3((unsigned)p.tiles * p.kv.n_kv * (rows / 4)), block, 0, s, p, rows);
 }
 
