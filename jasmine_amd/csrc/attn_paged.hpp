@@ -1079,7 +1079,7 @@ void paged_launch_as(const PagedAttnArgs &p, int rows, hipStream_t s)
     const dim3 grid((unsigned)p.tiles * p.nsplit * p.kv.n_kv), block(256);
     if (rows == 16) hipLaunchKernelGGL((paged_stream_kernel<D, CK, T>), grid, block, 0, s, p);
     else if (rows == 64) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 1>), grid, block, 0, s, p);
-    else if constexpr (sizeof(T) == 2 || D < 128) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 2>), grid, block, 0, s, p);
+    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((paged_tile_kernel<D, CK, T, 2>), grid, block, 0, s, p);
     if (p.nsplit > 1) hipLaunchKernelGGL((paged_merge_kernel<D, T>), dim3((unsigned)p.tiles * p.kv.n_kv * (rows / 4)), block, 0, s, p, rows);
 }
 

@@ -366,6 +366,17 @@ def test_attention_long(jas, dtype, cache, news, lens):
     within(y2, o, tolerance(o, mag, big, 64, max(lens), dtype))
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("heads,news,lens", [(32, [100, 0, 217, 64, 3, 216], [150, 0, 217, 300, 3, 400]), (32, [129, 500, 400, 1], [129, 700, 401, 90])])
+def test_attention_many_rows(jas, dtype, cache, heads, news, lens):
+    """Enough rows that every unit has a tile of 64 of them, or of 128."""
+    rng = np.random.default_rng(21)
+    c, cu, lens = filled(jas, rng, cache, news, lens, 16, heads, 32)
+    q = rounded(rng.standard_normal((int(cu[-1]), heads, 32)), dtype)
+    o, mag, big = R.attention(c, q, cu, lens, 0.2, 1, len(q))
+    within(attend(jas, c, q, cu, lens, 0.2, 1, dtype), o, tolerance(o, mag, big, 32, max(lens), dtype))
+
+
 @pytest.mark.parametrize("news,lens", [([1, 1], [700, 5]), ([20, 3], [300, 900]), ([40], [41])])
 def test_attention_any_bound(jas, news, lens):
     """The largest max_len there is: the results are within the same tolerance."""
