@@ -317,8 +317,8 @@ jas_status jas_kv_read(const jas_paged_kv *kv, void *d_k, void *d_v, int n, int6
  * JAS_F8E4M3; probabilities rounded to bf16, sums in fp32).
  * max_q: new tokens of the longest sequence, max_len: tokens of the longest (hosts' numbers, so
  * that the call reads nothing back; max_q only picks the kernel, lengths above max_len or a row of
- * the table are taken as that).  d_work: jas_attn_paged_workspace(...) bytes of the same arguments, 16-byte
- * aligned, no initialisation, NULL where that is 0; calls that share it must not overlap. */
+ * the table are taken as that).  d_work: jas_attn_paged_workspace(...) bytes of the same arguments or larger ones
+ * (H / n_kv, n_kv and dh alike), 16-byte aligned, no initialisation, NULL where that is 0; calls that share it must not overlap. */
 size_t jas_attn_paged_workspace(int n, int B, int H, int n_kv, int dh, int max_q, int max_len);
 jas_status jas_attn_paged(const void *d_q, void *d_o, const jas_paged_kv *kv, int n, int B, const int32_t *d_cu,
                           const int32_t *d_lens, int H, int max_q, int max_len, int64_t q_st, int64_t q_sh,
@@ -378,7 +378,7 @@ jas_status jas_argmax(const float *d_x, int n, int V, long ld, int32_t *d_out, j
  * Weights are formed in 64 bits and summed as whole numbers, so results do not depend on the
  * order of sums.  V up to 2^22, n up to 65535.  A top_k above 1024 but below V, a temperature of
  * infinity and a top_k or top_p that cuts among thousands of nearly equal logits take a slower
- * kernel, with the same result.  d_work: jas_sample_workspace(n, V) bytes, 16-byte aligned, no
+ * kernel, with the same result.  d_work: jas_sample_workspace(n, V) bytes (or for a larger n or V), 16-byte aligned, no
  * initialisation, NULL where that is 0; calls that share it must not overlap. */
 size_t jas_sample_workspace(int n, int V);
 jas_status jas_sample(const void *d_x, int n, int V, int64_t ld, const float *d_temp, const int32_t *d_top_k,

@@ -15,6 +15,10 @@ static int paged_cus()
     return n;
 }
 
+// Rounds of workgroups that tiles whose keys are split make, and the fewest keys of a split
+static constexpr int paged_rounds(int rows) { return rows == 16 ? 8 : rows == 64 ? 4 : 2; }
+static constexpr int paged_least(int rows) { return rows == 16 ? 128 : 256; }
+
 // Tiles of 16 rows stream the keys once for each tile, without LDS: for sequences whose new rows
 // (tokens times the query heads of a key head) fit one.  Otherwise tiles of 64 rows, or of 128, which
 // read fragments from LDS for twice the products but come in half the number, less evenly loaded.
@@ -44,17 +48,25 @@ static PagedPlan paged_plan(int n, int B, int H, int n_kv, int max_q, int max_le
     // splits: see paged_block.
     if (r.rows > 16 && full(r.rows) >= cus) r.chunk = std::max(max_len, 1), r.nsplit = 1;
     else {
-        const double share = (double)full(r.rows) * max_len / ((r.rows == 16 ? 8 : r.rows == 64 ? 4 : 2) * cus), least = r.rows == 16 ? 128 : 256;
-        r.chunk = (int)std::min(((long)std::max(least, std::min(share, (double)max_len)) + 127) / 128 * 128, 0x7fff0000L);
+        const double share = (double)full(r.rows) * max_len / (paged_rounds(r.rows) * cus);
+        r.chunk = (int)std::min(((long)std::max((double)paged_least(r.rows), std::min(share, (double)max_len)) + 127) / 128 * 128, 0x7fff0000L);
         r.nsplit = (int)std::max(1L, std::min(((long)max_len + r.chunk - 1) / r.chunk, 63L));
         if (r.nsplit > 1) r.nsplit |= 1;
     }
     return r;
 }
 
-static size_t paged_bytes(const PagedPlan &r, int n_kv, int D)
+// Bytes that hold the partial results of every call within the given numbers: fewer rows can need more
+// than many, whose keys are not split.  With x = max(B, n G / rows) n_kv there are at most 2 x tiles of a
+// head, of s = rounds cus / x + 1 splits, and one more to make them odd: 2 rounds cus + 4 x in all, where
+// x is below rounds cus (s = 1 otherwise) and for tiles of 64 and 128 below cus (not split otherwise).
+static size_t paged_bytes(int rows, int n, int B, int H, int n_kv, int D, int max_len)
 {
-    return r.nsplit > 1 ? (size_t)r.tiles * n_kv * r.nsplit * r.rows * (D + 4) * sizeof(float) : 0;
+    if (max_len <= paged_least(rows)) return 0;
+    const double cus = paged_cus(), rounds = paged_rounds(rows), G = H / n_kv;
+    const double x = std::min(std::max((double)B, n * G / rows) * n_kv, (rows == 16 ? rounds : 1.0) * cus);
+    const double parts = std::min(2 * rounds * cus + 4 * x, (n * G / rows + B) * n_kv * std::min(63.0, (double)max_len / paged_least(rows) + 2));
+    return (size_t)parts * rows * (D + 4) * sizeof(float);
 }
 
 } // namespace jas
@@ -66,9 +78,11 @@ extern "C" {
 size_t jas_attn_paged_workspace(int n, int B, int H, int n_kv, int dh, int max_q, int max_len)
 {
     if (n <= 0 || B <= 0 || H <= 0 || n_kv <= 0 || H % n_kv != 0 || dh <= 0 || max_q < 0 || max_len < 0) return 0;
-    // (of either type of rows)
-    return std::max(paged_bytes(paged_plan(n, B, H, n_kv, max_q, max_len, JAS_F32), n_kv, dh),
-                    paged_bytes(paged_plan(n, B, H, n_kv, max_q, max_len, JAS_BF16), n_kv, dh));
+    const double most = std::min((double)max_q, (double)n) * (H / n_kv);
+    size_t bytes = paged_bytes(16, n, B, H, n_kv, dh, max_len);
+    if (most > 16) bytes = std::max(bytes, paged_bytes(64, n, B, H, n_kv, dh, max_len));
+    if (most > 64) bytes = std::max(bytes, paged_bytes(128, n, B, H, n_kv, dh, max_len));
+    return bytes;
 }
 
 jas_status jas_attn_paged(const void *q, void *o, const jas_paged_kv *kv, int n, int B, const int32_t *cu, const int32_t *lens,

@@ -887,9 +887,9 @@ extern "C" {
 size_t jas_sample_workspace(int n, int V)
 {
     if (n <= 0 || V <= 0 || V > 1 << 22) return 0;
-    int C, chunk;
-    sample_chunks(n, V, C, chunk);
-    return (size_t)n * C * (NB * sizeof(unsigned long long) + 2 * sizeof(uint32_t));
+    // chunks of all rows, at most (sample_chunks), and of every call of fewer or shorter ones
+    const size_t rows = n, most = std::max(rows * ((V + 16383) / 16384), std::min(rows + 1023, rows * ((V + 4095) / 4096)));
+    return most * (NB * sizeof(unsigned long long) + 2 * sizeof(uint32_t));
 }
 
 jas_status jas_sample(const void *x, int n, int V, int64_t ld, const float *temp, const int32_t *top_k, const float *top_p,

@@ -273,7 +273,7 @@ def test_kv_bad_pages(jas):
 
 
 # ---------------------------------------------------------------- attention
-def attend(jas, c, q, cu, lens, scale, causal, dtype, max_q=None, max_len=None, n=None, pad=0, stream=None):
+def attend(jas, c, q, cu, lens, scale, causal, dtype, max_q=None, max_len=None, n=None, pad=0, stream=None, within=None):
     n = n if n is not None else int(cu[-1])
     H, D = q.shape[1:]
     st, sh = H * (D + pad) + pad, D + pad
@@ -284,10 +284,14 @@ def attend(jas, c, q, cu, lens, scale, causal, dtype, max_q=None, max_len=None, 
     max_q = max_q if max_q is not None else int(max(np.diff(cu)))
     max_len = max_len if max_len is not None else int(max(lens))
     size = jas.lib.jas_attn_paged_workspace(n, B, H, c.shape[1], D, max_q, max_len)
-    work = jas.to_device(np.full(max(size, 1), 255, np.uint8))  # NaN partials, if one is read unwritten
+    if within is not None:  # the workspace of a larger call
+        assert size <= within
+        size = within
+    work = jas.to_device(np.full(max(size, 1) + (1 << 20), 255, np.uint8))  # NaN partials, if one is read unwritten
     d_cu, d_lens = jas.to_device(cu), jas.to_device(lens)
     jas.check(jas.lib.jas_attn_paged(d_q.p, d_o.p, c.ref, n, B, d_cu.p, d_lens.p, H, max_q, max_len, st, sh, st, sh, scale, causal, dtype,
                                      work.p if size else None, stream))
+    assert np.all(work.numpy()[max(size, 1):] == 255)
     y = got(d_o, dtype)
     inner = np.ascontiguousarray(np.lib.stride_tricks.as_strided(y, (n, H, D), (4 * st, 4 * sh, 4)))
     mask = np.ones((n, st), bool)
@@ -375,6 +379,18 @@ def test_attention_many_rows(jas, dtype, cache, heads, news, lens):
     q = rounded(rng.standard_normal((int(cu[-1]), heads, 32)), dtype)
     o, mag, big = R.attention(c, q, cu, lens, 0.2, 1, len(q))
     within(attend(jas, c, q, cu, lens, 0.2, 1, dtype), o, tolerance(o, mag, big, 32, max(lens), dtype))
+
+
+@pytest.mark.parametrize("dtype,cache", [(F32, F32), (BF16, BF16)])
+def test_attention_steps_in_one_workspace(jas, dtype, cache):
+    """Smaller steps, whose keys are split where the largest's are not, in the largest's workspace."""
+    size = jas.lib.jas_attn_paged_workspace(600, 8, 32, 32, 32, 217, 900)
+    for news, lens in [([1], [900]), ([1] * 8, [900] * 8), ([30, 1], [900, 20]), ([217], [900]), ([100, 0, 217, 64, 3, 216], [150, 0, 217, 300, 3, 900])]:
+        rng = np.random.default_rng(22)
+        c, cu, lens = filled(jas, rng, cache, news, lens, 16, 32, 32)
+        q = rounded(rng.standard_normal((int(cu[-1]), 32, 32)), dtype)
+        o, mag, big = R.attention(c, q, cu, lens, 0.2, 1, len(q))
+        within(attend(jas, c, q, cu, lens, 0.2, 1, dtype, within=size), o, tolerance(o, mag, big, 32, max(lens), dtype))
 
 
 @pytest.mark.parametrize("news,lens", [([1, 1], [700, 5]), ([20, 3], [300, 900]), ([40], [41])])

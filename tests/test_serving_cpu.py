@@ -115,6 +115,19 @@ def test_workspaces(capi):
     assert all(g(n, V) >= n * 8 for n in (1, 7, 3000) for V in (1, 5000, 1 << 22))
 
 
+def test_workspace_of_a_larger_call(capi):
+    """Bytes for given numbers are enough for smaller ones: they never fall as a number grows."""
+    rng = np.random.default_rng(3)
+    upto = lambda hi: int(np.exp(rng.uniform(0, np.log(hi))))  # noqa: E731
+    for _ in range(3000):
+        n, B, max_q, max_len, V = upto(20000), upto(3000), upto(2000), upto(300000), upto(1 << 22)
+        g, kv = int(rng.choice([1, 2, 4, 7, 16])), int(rng.choice([1, 2, 8, 12, 32]))
+        less = [upto(v) for v in (n, B, max_q, max_len)]
+        f = capi.lib.jas_attn_paged_workspace
+        assert f(less[0], less[1], g * kv, kv, 64, less[2], less[3]) <= f(n, B, g * kv, kv, 64, max_q, max_len)
+        assert capi.lib.jas_sample_workspace(less[0], upto(V)) <= capi.lib.jas_sample_workspace(n, V)
+
+
 @pytest.mark.parametrize("n,B,H,n_kv,max_q", [(512, 512, 64, 8, 1), (4, 4, 32, 8, 1), (1 << 20, 1 << 20, 64, 64, 1), (5, 1, 8, 8, 5), (64, 2, 32, 8, 32)])
 def test_workspace_of_any_bound(capi, n, B, H, n_kv, max_q):
     """max_len only bounds: the largest one is as good as another, and 63 parts of a row are the most."""
