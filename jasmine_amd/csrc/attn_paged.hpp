@@ -23,6 +23,7 @@
 // weight of 0 times NaN) ends in a result that is not finite; such a row is computed again by
 // paged_row in plain fp32, which looks at no key that the row does not see.
 #pragma once
+#include "attn_paged_plan.hpp"
 #include "paged.hpp"
 #include "split.hpp"
 
@@ -45,12 +46,6 @@ struct PagedAttnArgs {
     float *part;                // nsplit > 1: rows of D means, then exponent base and sum
 };
 
-// How a call is launched
-struct PagedPlan {
-    int rows;  // of a tile: 16 (its waves share the keys), 64 or 128
-    long tiles;
-    int nsplit, chunk;
-};
 // One call's kernels for head dim 32, 64, 128
 void paged_launch_32(const PagedAttnArgs &p, int rows, int cache, int dtype, hipStream_t s);
 void paged_launch_64(const PagedAttnArgs &p, int rows, int cache, int dtype, hipStream_t s);

@@ -813,3 +813,16 @@ def test_results_repeat(jas):
         assert np.array_equal(attend(jas, c, q, cu, lens, 0.09, 1, BF16), first)
         again = draw(jas, x, F32, top_p=[0.9] * 3, u=u)
         assert np.array_equal(again[0], ids[0]) and np.array_equal(again[1], ids[1])
+
+
+@pytest.mark.parametrize("dtype,cache,news,lens,heads,g,max_q", [
+    (BF16, BF16, [32] * 8 + [137], [600, 14000, 64, 9000, 33, 2000, 500, 40, 14619], 1, 3, 156),  # tiles of 128 rows, tens of splits
+    (BF16, I8, [3, 2, 1] * 11 + [1, 1, 15], [700, 7000, 90] * 11 + [60, 70, 7297], 1, 7, 2),  # of 16, max_q below the longest
+    (F32, BF16, [1] * 412, [300, 5, 90, 2] * 102 + [640, 1, 17, 641], 1, 16, 1)])
+def test_attention_splits_in_its_workspace(jas, dtype, cache, news, lens, heads, g, max_q):
+    """Shares of the keys just above a multiple of 128: the last sequence's last splits end within the workspace."""
+    rng = np.random.default_rng(len(lens))
+    c, cu, lens = filled(jas, rng, cache, news, lens, 64, heads, 64)
+    q = rounded(rng.standard_normal((int(cu[-1]), g * heads, 64)), dtype)
+    o, mag, big = R.attention(c, q, cu, lens, 0.125, 1, len(q))
+    within(attend(jas, c, q, cu, lens, 0.125, 1, dtype, max_q=max_q), o, tolerance(o, mag, big, 64, max(lens), dtype))
