@@ -1021,7 +1021,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
 }
 
 // Joins the splits of a tile's rows, one wave a row: lane i weighs split i (nsplit <= 64), then the
-// wave adds the means of the splits that have weight, sixteen in flight.  (6 us of the 71.5 above; 9 of
+// wave adds the means of the splits that saw a key, sixteen in flight (one of no weight too: 0 times NaN).  (6 us of the 71.5 above; 9 of
 // int8's 73, whose rows have 63 splits.)
 template <int D, typename T>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs p, int M)
@@ -1042,7 +1042,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs p,
     float wt = l != 0.f ? paged_exp2(m - base) * l : 0.f;
     const float ll = wave_sum(wt);
     wt *= ll != 0.f ? 1.0f / ll : 0.f;
-    unsigned long long left = __builtin_amdgcn_ballot_w64(wt != 0.f);  // (a NaN weight too)
+    unsigned long long left = __builtin_amdgcn_ballot_w64(l != 0.f);  // (a NaN sum too)
     const int d = lane * E;
     float v[E];
 #pragma unroll

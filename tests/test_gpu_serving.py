@@ -826,3 +826,26 @@ def test_attention_splits_in_its_workspace(jas, dtype, cache, news, lens, heads,
     q = rounded(rng.standard_normal((int(cu[-1]), g * heads, 64)), dtype)
     o, mag, big = R.attention(c, q, cu, lens, 0.125, 1, len(q))
     within(attend(jas, c, q, cu, lens, 0.125, 1, dtype, max_q=max_q), o, tolerance(o, mag, big, 64, max(lens), dtype))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_attention_weightless_split_keeps_nan(jas, dtype, cache, new, bad):
+    """A value that is not finite, of a key whose weight is nothing beside other splits' keys: 0 times it is NaN, as in one split."""
+    rng = np.random.default_rng(51)
+    dh, L = 64, 5000
+    cu, lens, table, pages = batch(rng, [new], [L], 16)
+    c = R.Cache(jas, cache, pages, 1, 16, dh, table)
+    k, v = rng.standard_normal((2, L, 1, dh)).astype(np.float32)
+    k[:600] -= 30  # (scores lower by some 300: no fp32 weight)
+    v[10, 0, 3] = bad
+    whole = np.array([0, L], np.int32)
+    jas.check(jas.lib.jas_kv_append(c.ref, hold(put(jas, k, F32)), hold(put(jas, v, F32)), L, dh, dh, 1, hold(jas.to_device(whole)), hold(jas.to_device(lens)), F32, None))
+    c.put(k, v, whole, lens)
+    q = rounded(np.abs(rng.standard_normal((new, 2, dh))) + 0.5, dtype)
+    o, mag, big = R.attention(c, q, cu, lens, 0.125, 1, new)
+    y = attend(jas, c, q, cu, lens, 0.125, 1, dtype)
+    assert not np.isfinite(o[:, :, 3]).any() and not np.isfinite(y[:, :, 3]).any()
+    fine = np.isfinite(o)
+    within(np.where(fine, y, 0), np.where(fine, o, 0), np.where(fine, tolerance(o, mag, big, dh, L, dtype), 0))
