@@ -923,16 +923,17 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[j][a][r] = __builtin_fmaf(s[j][a][r], sl2, -mb[a]);
-            // The base moves only when a row's running maximum leaves [mb - 64, mb + 8]: p stays below
-            // 2^8, numerator and sum share the base, and the result is unchanged.  Each lane tests
-            // its own maximum; the row's is formed only when one trips.
+            // The base is the row's maximum over the first tile in which it sees a key, and moves only when its
+            // running maximum passes mb + 8: p stays below 2^8 and the largest at or above 1, numerator and
+            // sum share the base, and the result is unchanged.  Each lane tests its own maximum; the row's is
+            // formed only when one trips.
             const float m_prev = m_lane[a];
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
                 m_lane[a] = fmaxf(fmaxf(m_lane[a], fmaxf(s[j][a][0], s[j][a][1])), fmaxf(s[j][a][2], s[j][a][3]));
-            if (__builtin_amdgcn_ballot_w64(m_lane[a] > 8.f || (m_lane[a] < -64.f && m_lane[a] != -INFINITY))) {
+            if (__builtin_amdgcn_ballot_w64(m_lane[a] > 8.f || (m_prev == -INFINITY && m_lane[a] != -INFINITY))) {
                 const float row_prev = paged_max_rows(m_prev), row = paged_max_rows(m_lane[a]);
-                if (row > 8.f || (row < -64.f && row != -INFINITY)) {
+                if (row > 8.f || (row_prev == -INFINITY && row != -INFINITY)) {
                     // nothing accumulated yet (row_prev = -inf): factor 0, not a 2^-row that overflows
                     const float corr = row_prev == -INFINITY ? 0.f : paged_exp2(-row);
                     mb[a] += row;

@@ -849,3 +849,25 @@ def test_attention_weightless_split_keeps_nan(jas, dtype, cache, new, bad):
     assert not np.isfinite(o[:, :, 3]).any() and not np.isfinite(y[:, :, 3]).any()
     fine = np.isfinite(o)
     within(np.where(fine, y, 0), np.where(fine, o, 0), np.where(fine, tolerance(o, mag, big, dh, L, dtype), 0))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 24])
+@pytest.mark.parametrize("level", [-60, -40, 30])
+def test_attention_levels_and_magnitudes(jas, dtype, cache, new, level):
+    """Rows whose scores all lie far from 0 (in powers of two), over small and large values: weights are relative to the row's own
+    maximum, and numbers near the end of fp32 keep their accuracy."""
+    rng = np.random.default_rng(53)
+    dh, L = 64, 90
+    cu, lens, table, pages = batch(rng, [new], [L], 16)
+    q = rounded(rng.uniform(0.9, 1.1, (new, 2, dh)), dtype)
+    k = (level / (dh * 0.125 * 1.4427) + 0.1 * rng.standard_normal((L, 1, dh))).astype(np.float32)
+    unit = np.clip(rng.standard_normal((L, 1, dh)), -1.9, 1.9)
+    for mag in (2.0 ** -100, 1.0, 2.0 ** 100):
+        c = R.Cache(jas, cache, pages, 1, 16, dh, table)
+        v = (unit * mag).astype(np.float32)
+        whole = np.array([0, L], np.int32)
+        jas.check(jas.lib.jas_kv_append(c.ref, hold(put(jas, k, F32)), hold(put(jas, v, F32)), L, dh, dh, 1, hold(jas.to_device(whole)), hold(jas.to_device(lens)), F32, None))
+        c.put(k, v, whole, lens)
+        o, m, big = R.attention(c, q, cu, lens, 0.125, 1, new)
+        within(attend(jas, c, q, cu, lens, 0.125, 1, dtype), o, tolerance(o, m, big, dh, L, dtype))
