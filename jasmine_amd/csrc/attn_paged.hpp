@@ -13,7 +13,8 @@
 //
 // fp32 rows: q and p as three bf16 parts each (exact, split.hpp), and fp32 cache values too, so
 // that 3 or 6 products make fp32 accuracy.  8-bit codes are bf16 numbers exactly; a key's scale
-// multiplies its scores, a value's scale its weight.  bf16 rows: p as one bf16 number where the sum
+// multiplies its scores, a value's scale times 2^16 its weight (so that the weight's lower parts are
+// bf16 numbers too, whose last bit is 2^-133, where scales go down to 2^-126).  bf16 rows: p as one bf16 number where the sum
 // of the weights can be taken of what was rounded (by a product with ones: a row that one key
 // dominates then loses nothing), and as two where it cannot (scaled weights) or where the products
 // are for nothing (few rows): one part alone left results 1.5 times as far from 64 bits as their own
@@ -599,7 +600,7 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
         }
         float vsc[8];
         if (EIGHT) {
-            s_sc[w][0][lane & 31] = ks, s_sc[w][1][lane & 31] = vs;
+            s_sc[w][0][lane & 31] = ks, s_sc[w][1][lane & 31] = vs * SPLIT_SCALE;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -676,7 +677,7 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
     const float base = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
     for (int k = 0; k < 4; ++k) ll += s_l[k][r16] * paged_exp2(s_m[k][r16] - base);
-    const float f = (ll != 0.f ? paged_exp2(m - base) / ll : 0.f) * (NK == 3 ? SPLIT_UNSCALE : 1.f);
+    const float f = (ll != 0.f ? paged_exp2(m - base) / ll : 0.f) * (NK == 3 || EIGHT ? SPLIT_UNSCALE : 1.f);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -813,7 +814,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
         }
     };
     auto lstore = [&](int buf, int at, unsigned long long valid) {
-        if (EIGHT && w == 0) s_sc[at][0][lane] = ks, s_sc[at][1][lane] = (valid >> lane & 1) ? vs : 0.f;
+        if (EIGHT && w == 0) s_sc[at][0][lane] = ks, s_sc[at][1][lane] = (valid >> lane & 1) ? vs * SPLIT_SCALE : 0.f;
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             u32x4 pl[NK];
@@ -975,7 +976,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
     for (int a = 0; a < NQ; ++a) {
         const int r = wr + 16 * a + r16;
         const float ll = ONES ? lacc[a][0] : paged_sum_rows(l[a]);
-        const float inv = (ll != 0.f ? 1.0f / ll : 0.f) * (NK == 3 ? SPLIT_UNSCALE : 1.f);
+        const float inv = (ll != 0.f ? 1.0f / ll : 0.f) * (NK == 3 || EIGHT ? SPLIT_UNSCALE : 1.f);
         bool bad = !(ll <= FLT_MAX);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {

@@ -871,3 +871,25 @@ def test_attention_levels_and_magnitudes(jas, dtype, cache, new, level):
         c.put(k, v, whole, lens)
         o, m, big = R.attention(c, q, cu, lens, 0.125, 1, new)
         within(attend(jas, c, q, cu, lens, 0.125, 1, dtype), o, tolerance(o, m, big, dh, L, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cache", [BF16, I8, F8])
+@pytest.mark.parametrize("new", [1, 24])
+@pytest.mark.parametrize("mag", [2.0 ** -124, 2.0 ** -118, 2.0 ** -110, 2.0 ** 112, 2.0 ** 120])
+def test_attention_small_cache_magnitudes(jas, dtype, cache, new, mag):
+    """Caches of fewer bits that hold values near both ends of fp32 (8 bits: scales down to 2^-126): no part of a weight is lost."""
+    rng = np.random.default_rng(57)
+    dh, L = 64, 70
+    cu, lens, table, pages = batch(rng, [new], [L], 16)
+    c = R.Cache(jas, cache, pages, 1, 16, dh, table)
+    k, v = rng.standard_normal((2, L, 1, dh)).astype(np.float32)
+    v = (np.clip(v, -1.9, 1.9) * mag).astype(np.float32)
+    whole = np.array([0, L], np.int32)
+    jas.check(jas.lib.jas_kv_append(c.ref, hold(put(jas, k, F32)), hold(put(jas, v, F32)), L, dh, dh, 1, hold(jas.to_device(whole)), hold(jas.to_device(lens)), F32, None))
+    c.put(k, v, whole, lens)
+    q = rounded(rng.standard_normal((new, 2, dh)), dtype)
+    o, m, big = R.attention(c, q, cu, lens, 0.125, 1, new)
+    # (a bf16 result below 2^-126 is rounded to a multiple of 2^-133; sums of fp32 products to multiples of 2^-149)
+    least = 2.0 ** -134 if dtype == BF16 else 0.0
+    within(attend(jas, c, q, cu, lens, 0.125, 1, dtype), o, tolerance(o, m, big, dh, L, dtype) + least + 2.0 ** -149 * (L + 8))
