@@ -854,7 +854,11 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
 #pragma unroll
         for (int c = 0; c < NC; ++c) oacc[c][a] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
-    const float sl2 = p.scale_log2 * (NP == 3 ? SPLIT_UNSCALE : 1.f) * (NK == 3 ? SPLIT_UNSCALE : 1.f);
+    // Scores are masked before they are scaled (after it, the same work took 44.4 us for 38.3 of attn_chunk_f32), so
+    // a masked score is what the scale makes -inf: of the other sign under a negative one, and 2^-126 stands
+    // for 0, which leaves scores of up to 2^60 their weight of 1.
+    const float scaled = p.scale_log2 * (NP == 3 ? SPLIT_UNSCALE : 1.f) * (NK == 3 ? SPLIT_UNSCALE : 1.f);
+    const float sl2 = scaled == 0.f ? 0x1p-126f : scaled, none = sl2 < 0.f ? INFINITY : -INFINITY;
     const bf16x8 ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
 
     if (k_lo < k_hi) {
@@ -917,7 +921,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs 
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[j][a][r] = (see >> (16 * j + r) & 1) && 16 * j + r < lim ? s[j][a][r] : -INFINITY;
+                    for (int r = 0; r < 4; ++r) s[j][a][r] = (see >> (16 * j + r) & 1) && 16 * j + r < lim ? s[j][a][r] : none;
             }
             // exponent units relative to the base: p = 2^s below
 #pragma unroll

@@ -893,3 +893,20 @@ def test_attention_small_cache_magnitudes(jas, dtype, cache, new, mag):
     # (a bf16 result below 2^-126 is rounded to a multiple of 2^-133; sums of fp32 products to multiples of 2^-149)
     least = 2.0 ** -134 if dtype == BF16 else 0.0
     within(attend(jas, c, q, cu, lens, 0.125, 1, dtype), o, tolerance(o, m, big, dh, L, dtype) + least + 2.0 ** -149 * (L + 8))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("news,lens", [([1, 1], [70, 333]), ([40, 7], [90, 33]), ([70], [300]), ([20], [2500])])
+def test_attention_scale_sign(jas, dtype, cache, news, lens):
+    """Scales below zero, and of zero: the latter takes the same path as queries of zero, to the bit (a matrix instruction's sums are not
+    the same bits with their signs changed)."""
+    rng = np.random.default_rng(59)
+    c, cu, lens = filled(jas, rng, cache, news, lens, 16, 2, 64)
+    q = rounded(rng.standard_normal((int(cu[-1]), 6, 64)), dtype)
+    for causal in (1, 0):
+        o, mag, big = R.attention(c, q, cu, lens, -0.125, causal, len(q))
+        within(attend(jas, c, q, cu, lens, -0.125, causal, dtype), o, tolerance(o, mag, big, 64, max(lens), dtype))
+        zero = attend(jas, c, q, cu, lens, 0.0, causal, dtype)
+        assert np.array_equal(zero, attend(jas, c, 0 * q, cu, lens, 0.125, causal, dtype))
+        o, mag, big = R.attention(c, q, cu, lens, 0.0, causal, len(q))
+        within(zero, o, tolerance(o, mag, big, 64, max(lens), dtype))
