@@ -144,7 +144,7 @@ __device__ __forceinline__ bool find_token(const BatchView &bt, const int32_t *c
     }
     b = lo;
     if (b >= bt.B || cu[b] > tok) return false;
-    pos = bt.lens[b] - (cu[b + 1] - tok);
+    pos = max(0, bt.lens[b]) - (cu[b + 1] - tok);  // (both at least 0: a length of -2^31 does not wrap)
     return true;
 }
 

@@ -910,3 +910,19 @@ def test_attention_scale_sign(jas, dtype, cache, news, lens):
         assert np.array_equal(zero, attend(jas, c, 0 * q, cu, lens, 0.125, causal, dtype))
         o, mag, big = R.attention(c, q, cu, lens, 0.0, causal, len(q))
         within(zero, o, tolerance(o, mag, big, 64, max(lens), dtype))
+
+
+def test_kv_lengths_below_any_position(jas):
+    """A length of -2^31: every position is below 0, however many rows the sequence has."""
+    dh, page, n = 32, 1 << 20, 70000
+    table = np.zeros((1, 2048), np.int32)  # a row that holds 2^31 positions, all of them in page 0
+    cache = jas.DeviceArray(page * dh, np.uint8).zero()
+    scales = jas.DeviceArray(page, np.float32).zero()
+    d_table, d_cu, d_lens = jas.to_device(table), jas.to_device(np.array([0, n], np.int32)), jas.to_device(np.array([-2 ** 31], np.int32))
+    kv = jas.PagedKv(cache.ptr, cache.ptr, scales.ptr, scales.ptr, d_table.ptr, page * dh, page * dh, dh, 2048, 2048, I8, 1, page, 1, dh)
+    rows = jas.to_device(np.ones((n, dh), np.float32))
+    jas.check(jas.lib.jas_kv_append(R.C.byref(kv), rows.p, rows.p, n, dh, dh, 1, d_cu.p, d_lens.p, F32, None))
+    assert not cache.numpy().any() and not scales.numpy().any()
+    scales.upload(np.ones(page, np.float32)), cache.upload(np.ones(page * dh, np.uint8))
+    jas.check(jas.lib.jas_kv_read(R.C.byref(kv), rows.p, None, n, dh, dh, 1, d_cu.p, d_lens.p, F32, None))
+    assert not rows.numpy().any()
