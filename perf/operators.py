@@ -314,6 +314,15 @@ def _plain_sample(s):
 
 
 # ------------------------------------------------------------------ the library's calls
+def _workspace(size, kept=[]):  # (one for all calls: they follow each other on the library's stream)
+    """Memory of the library's allocation: torch hands back blocks that its own stream's kernels may still use, and nothing
+    orders those with the library's stream."""
+    from jasmine_amd.capi import DeviceArray
+    if not kept or kept[0].nbytes < size:
+        kept[:] = [DeviceArray(max(1, size), np.uint8)]
+    return kept[0]
+
+
 def _own(s):
     from jasmine_amd.capi import PagedKv, check, lib
     c, op = s["case"], s["case"]["op"]
@@ -326,9 +335,9 @@ def _own(s):
     if op == "sample":
         n, v = c["n"], c["vocab"]
         if "work" not in s:
-            s["work"] = torch.empty(max(1, lib.jas_sample_workspace(n, v)), dtype=torch.uint8, device=DEV)
+            s["work"] = _workspace(lib.jas_sample_workspace(n, v))
         check(lib.jas_sample(p("x"), n, v, v, p("temp"), p("top_k"), p("top_p"), p("min_p"), p("u"), p("ids"), p("logp"),
-                             CODES[c["dtype"]], p("work"), None))
+                             CODES[c["dtype"]], s["work"].p, None))
         return {"ids": s["ids"], "logp": s["logp"]}
     hk, d, page, eight = c["kv_heads"], c["dh"], c["page"], c["cache"] in QMAX
     if "kv" not in s:
@@ -343,10 +352,9 @@ def _own(s):
         return {"k": s["k_out"], "v": s["v_out"], **({"k_scale": s["k_scale"], "v_scale": s["v_scale"]} if eight else {})}
     h = c["heads"]
     if "work" not in s:
-        s["work"] = torch.empty(max(1, lib.jas_attn_paged_workspace(s["n"], c["b"], h, hk, d, s["most"], s["longest"])),
-                                dtype=torch.uint8, device=DEV)
+        s["work"] = _workspace(lib.jas_attn_paged_workspace(s["n"], c["b"], h, hk, d, s["most"], s["longest"]))
     check(lib.jas_attn_paged(p("q"), p("o"), kv, s["n"], c["b"], p("cu"), p("lens"), h, s["most"], s["longest"], h * d, d, h * d, d,
-                             1.0 / math.sqrt(d), 1, CODES[c["dtype"]], p("work"), None))
+                             1.0 / math.sqrt(d), 1, CODES[c["dtype"]], s["work"].p, None))
     return s["o"]
 
 
