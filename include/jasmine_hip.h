@@ -299,7 +299,8 @@ typedef struct {
  *
  * Writes the new tokens' keys and values (device, JAS_F32 or JAS_BF16, token stride st, head
  * stride sh, in elements, both tensors alike) to the cache.  Two rows of one call must not name
- * the same slot (a page that two sequences share is written by one of them at most). */
+ * the same slot (a page that two sequences share is written by one of them at most; strides under which
+ * rows of the cache overlap are for reading only). */
 jas_status jas_kv_append(const jas_paged_kv *kv, const void *d_k, const void *d_v, int n, int64_t st, int64_t sh,
                          int B, const int32_t *d_cu, const int32_t *d_lens, int dtype, jas_stream_t stream);
 /* Reads them back, widened or rounded to dtype (JAS_F32 or JAS_BF16).  d_cu may count whole
@@ -311,10 +312,12 @@ jas_status jas_kv_read(const jas_paged_kv *kv, void *d_k, void *d_v, int n, int6
  * O = softmax(scale Q K^T) V over the keys at positions up to the row's own (causal = 1) or over
  * all of its sequence (0).  One row per sequence is a decode step, more a chunk of a prompt; both
  * may be mixed in a call.  Query head h of H reads key head h / (H / n_kv).  Q and O: row stride
- * st, head stride sh (elements); O must not overlap Q.  A row that sees no key is zeros.  Keys
- * past a row's position do not reach it, whatever they hold.
+ * st, head stride sh (elements); O must not overlap Q.  A row that sees no key is zeros, and so is one
+ * whose scores are all -inf.  Keys past a row's position do not reach it, whatever they hold.  Weights
+ * below 2^-126 of a row's largest count as 0 (times an infinity or NaN: NaN).
  * dtype JAS_F32 (over a cache of any type: fp32 accuracy) or JAS_BF16 (over JAS_BF16, JAS_I8 and
- * JAS_F8E4M3; probabilities rounded to bf16, sums in fp32).
+ * JAS_F8E4M3; probabilities rounded to bf16, sums in fp32: to one bf16 number in a call of chunks over
+ * JAS_BF16, to two where max_q (H / n_kv) is at most 16 or the cache is of 8 bits).
  * max_q: new tokens of the longest sequence, max_len: tokens of the longest (hosts' numbers, so
  * that the call reads nothing back; max_q only picks the kernel, lengths above max_len or a row of
  * the table are taken as that).  d_work: jas_attn_paged_workspace(...) bytes of the same arguments or larger ones

@@ -106,8 +106,8 @@ __device__ __forceinline__ int paged_tile(const PagedAttnArgs &p, int x, int &b,
 // <= 256): each thread adds the tiles of the sequences before its own.  Workgroups start in the order
 // of their ids; where two fit on a unit, i and i + cus share one, so the second cus of them are
 // taken from the light end.  24 sequences of up to 2048 keys, chunks of up to 256
-// beside single tokens, bf16: 96 -> 77 us; 4 chunks of up to 512 over up to 4096 keys, bf16:
-// 137 -> 126.
+// beside single tokens, bf16: 96 us unsorted, 77 sorted; 4 chunks of up to 512 over up to 4096 keys, bf16:
+// 137, 126 (121 since the exponents' base is a row's own maximum).
 template <int M>
 __device__ __forceinline__ int paged_tile_sorted(const PagedAttnArgs &p, int x, int &b, PagedSeq &sq)
 {
@@ -716,10 +716,12 @@ __global__ void __launch_bounds__(256, (stream_waves<D, CK, T>)) paged_stream_ke
 // share out the staging, 4 chunks of up to 512 over up to 4096 keys take 181 us over int8 and 132 over bf16,
 // with 32 and four 171 and 126; with 32 and eight, tiles of 256 rows are too few to even out: 260.  Scales of
 // values are read from LDS where they are used: held in registers (two fragments in flight): 258.
-// Those chunks over bf16 are 73.6 GFLOP: 587 TFLOP/s, where a large bf16 product of a library reaches 1208.
-// The matrix cores are busy 0.25 of the time that all units are held, the vector ALU (softmax, staging)
-// 0.32, one mostly while the other waits; the rest is two tiles a unit of unequal length.  Two groups of
-// waves that share a tile's keys (142 us), keys split so that tiles are equal (158), two sets of
+// Those chunks over bf16 are 73.6 GFLOP in 121 us, alone and back to back: 609 TFLOP/s, where a large bf16
+// product of a library reaches 1208; over int8 168, e4m3 161.  A unit is held for 0.77 of the kernel (two
+// tiles of unequal length each); of that time the matrix cores are busy 0.32 and the vector ALU (softmax,
+// staging) 0.36.  Neither is full: a wave's products and its softmax take turns, and the one other
+// wave of its SIMD does not fill the gaps (0.29 of a wave's cycles wait for memory, LDS or the barrier, 0.32 to
+// issue).  Two groups of waves that share a tile's keys (142 us), keys split so that tiles are equal (158), two sets of
 // registers for the staged rows (no change) and longer rings (they spill: 151) were slower.
 template <int D, int CK, typename T, int NQ>
 __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttnArgs p)

@@ -23,12 +23,13 @@ constexpr int paged_least(int rows) { return rows == 16 ? 128 : 256; }
 // Tiles of 16 rows stream the keys once for each tile, without LDS: for sequences whose new rows
 // (tokens times the query heads of a key head) fit one.  Otherwise tiles of 64 rows, or of 128, which
 // read fragments from LDS for twice the products but come in half the number, less evenly loaded.
-// (us, tiles of 128 and of 64; lengths spread up to what is named, heads of 128 but as said)
-//   fp32 rows, 12 heads of 64: 16 x up to 200 tokens over 1024 keys 98, 55; 8 x 1024 92, 82; 2 x 333 over 2001
-//     39.5, 38.7; 500 over 8000 93, 105: always 64
-//   bf16 rows, 128 give a workgroup to every unit: 4 x 512 over 4096 125, 142; 24 x 256 over 2048, e4m3 92, 98
-//   only 64 do, with some over: 2 x 512 over 4096 111, 88, int8 138, 112; 6 x 300 over 2048, 16 heads of 64 71, 48
-//   neither does: 512 over 8192, int8 139, 208; 300 over 6000 45, 52
+// (us, tiles of 128 and of 64; lengths spread up to what is named, 32 query heads of 128 on 8 but as said)
+//   fp32 rows, 12 heads of 64: 16 x up to 200 tokens over 1024 keys 98, 55; 8 x 1024 92, 81; 2 x 333 over 2001
+//     39.5, 38.5; 500 over 8000 93, 102: always 64
+//   bf16 rows, 128 give a workgroup to every unit: 4 x 512 over 4096 121, 138; 24 x 256 beside single tokens over
+//     2048, e4m3 88, 94
+//   only 64 do, with some over: 2 x 512 over 4096 106, 86, int8 135, 112; 6 x 300 over 2048, 16 heads of 64, int8 68, 48
+//   neither does: 512 over 8192, int8 135, 212; 300 over 6000 80, 80
 inline PagedPlan paged_plan(int n, int B, int H, int n_kv, int max_q, int max_len, int dtype, long cus)
 {
     PagedPlan r;
@@ -43,10 +44,11 @@ inline PagedPlan paged_plan(int n, int B, int H, int n_kv, int max_q, int max_le
     // Tiles of 16 rows: eight rounds of one workgroup a unit (32 sequences of 1024 to 4096 keys, 8
     // heads, bf16: 75.2, 71.0, 72.1, 78.9 us at 6, 8, 12, 16).  Larger tiles are bound by the matrix
     // cores and their partial results are large: split only where units would be left without one
-    // (2 x 333 rows over 2001 keys, 12 heads of 64, fp32: 82, 38.7 us unsplit and split; 4 chunks of 512
-    // over 4096, bf16: 125, 163), those of 64 into four rounds (that fp32: 42.4, 38.8, 38.7 at 2, 3, 4),
-    // those of 128 into two (512 over 8192, int8: 172, 139, 169, 150 at 1.5, 2, 3, 4).  An odd number of
-    // splits: see paged_block.
+    // (2 x 333 rows over 2001 keys, 12 heads of 64, fp32: 81, 38.5 us unsplit and split; 4 chunks of 512
+    // over 4096, bf16: 121, 167), those of 64 into four rounds (that fp32: 41.7, 38.7, 38.3 at 2, 3, 4),
+    // those of 128 into two (512 over 8192, int8: 169, 135, 161, 143 at 1.5, 2, 3, 4).  An odd number of
+    // splits: see paged_block.  One plan for the whole call: beside chunks that fill the chip a single token's
+    // keys are not split either (3 chunks of 512 over 4096 and one token over 32768 keys: 839 us, 120 and 36 apart).
     if (r.rows > 16 && full(r.rows) >= cus) r.chunk = std::max(max_len, 1), r.nsplit = 1;
     else {
         // (a fraction of a key counts: a chunk below the share makes more splits than paged_bytes allows for)

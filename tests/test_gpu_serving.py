@@ -926,3 +926,28 @@ def test_kv_lengths_below_any_position(jas):
     scales.upload(np.ones(page, np.float32)), cache.upload(np.ones(page * dh, np.uint8))
     jas.check(jas.lib.jas_kv_read(R.C.byref(kv), rows.p, None, n, dh, dh, 1, d_cu.p, d_lens.p, F32, None))
     assert not rows.numpy().any()
+
+
+@pytest.mark.parametrize("dtype,cache", [(F32, F32), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("new,L", [(1, 70), (24, 70), (1, 3000), (20, 3000)])
+def test_attention_scores_of_minus_infinity(jas, dtype, cache, new, L):
+    """Rows whose scores are all -inf are zeros, as rows that see no key are; beside finite scores, -inf ones have no weight."""
+    rng = np.random.default_rng(61)
+    dh = 64
+    cu, lens, table, pages = batch(rng, [new], [L], 16)
+    q = rounded(np.abs(rng.standard_normal((new, 2, dh))) + 0.5, dtype)
+    for finite in (0, 3):
+        c = R.Cache(jas, cache, pages, 1, 16, dh, table)
+        k, v = rng.standard_normal((2, L, 1, dh)).astype(np.float32)
+        k[:L - new + 1 - finite] = -np.inf
+        k[L - new + 1:] = -np.inf
+        whole = np.array([0, L], np.int32)
+        jas.check(jas.lib.jas_kv_append(c.ref, hold(put(jas, k, F32)), hold(put(jas, v, F32)), L, dh, dh, 1, hold(jas.to_device(whole)), hold(jas.to_device(lens)), F32, None))
+        c.put(k, v, whole, lens)
+        y = attend(jas, c, q, cu, lens, 0.125, 1, dtype)
+        if finite:
+            o, mag, big = R.attention(c, q, cu, lens, 0.125, 1, new)
+            big = (np.abs(q).max() * dh * 0.125 * 6) * np.ones_like(big)  # (of the finite scores: |k| < 6)
+            within(y, o, tolerance(o, mag, big, dh, L, dtype))
+        else:
+            assert np.all(y == 0)
